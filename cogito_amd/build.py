@@ -34,8 +34,10 @@ HIP_FLAGS = [
 # contraction of a*b+c into fma).  decoder.hip is among them so that RoPE's
 # x0 c - x1 s rounds twice, as the reference's CPU code does, whatever the
 # surrounding code looks like (with contraction the backend fuses such pairs,
-# in the inlined sin / cos / pow too, depending on the code's layout).
-EXACT_FP = {"accept.hip", "int4.hip", "filter.hip", "tree.hip", "decoder.hip"}
+# in the inlined sin / cos / pow too, depending on the code's layout).  paged.hip
+# for its append, whose codes have to be the same bits as the contiguous cache's.
+EXACT_FP = {"accept.hip", "int4.hip", "filter.hip", "tree.hip", "decoder.hip",
+            "paged.hip"}
 C_FLAGS = ["-O2", "-fPIC", "-std=c11", "-Wall", "-Wextra", "-Wno-unused-parameter",
            # a call to an undeclared function (e.g. POSIX strdup under C11)
            # would truncate a returned pointer to int

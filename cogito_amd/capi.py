@@ -128,12 +128,33 @@ class CgxModelConfig(C.Structure):
     ]
 
 
+class CgxKvPagedInt4(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p),
+        ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("num_layers", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int),
+        ("n_heads", C.c_int), ("head_dim", C.c_int), ("group_size", C.c_int),
+    ]
+
+
+class CgxPagedStep(C.Structure):
+    _fields_ = [
+        ("seqs", C.c_int), ("rows", C.c_int), ("max_rows", C.c_int), ("table_ld", C.c_int),
+        ("kv_old", C.c_void_p), ("kv_keep", C.c_void_p), ("rows_new", C.c_void_p),
+        ("table_old", C.c_void_p), ("table", C.c_void_p), ("row_begin", C.c_void_p),
+        ("row_seq", C.c_void_p), ("row_pos", C.c_void_p), ("row_slot", C.c_void_p),
+        ("kv_len", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
 PT = C.POINTER(CgTensor)
 PQ = C.POINTER(CgTensorQuant)
 PKV = C.POINTER(CgKvCacheInt4)
 PTREE = C.POINTER(CgTokenTree)
 PDEC = C.POINTER(CgSpeculativeDecoder)
 PPARAMS = C.POINTER(CgFlashAttnParams)
+PPAGED = C.POINTER(CgxKvPagedInt4)
+PSTEP = C.POINTER(CgxPagedStep)
 VP = C.c_void_p
 I = C.c_int
 F = C.c_float
@@ -278,6 +299,16 @@ SIGNATURES: dict[str, tuple] = {
     "cgx_kv_cache_int4_set_len": (I, [PKV, I]),
     "cgx_attention_int4_kv_dev": (I, [VP, I, I, PKV, I, I, VP, VP]),
     "cgx_attention_int4_kv_batch_dev": (I, [VP, I, I, I, PKV, I, VP, I, VP, I, VP]),
+    # paged INT4 KV cache and serving steps
+    "cgx_kv_paged_int4_new": (PPAGED, [I, I, I, I, I, I]),
+    "cgx_kv_paged_int4_free": (None, [PPAGED]),
+    "cgx_paged_plan_dev": (I, [PSTEP, I, I, VP, VP, VP]),
+    "cgx_kv_paged_append_dev": (I, [PPAGED, I, PSTEP, VP, I, I, VP, I, VP]),
+    "cgx_kv_paged_gather_dev": (I, [PPAGED, I, VP, I, VP, VP]),
+    "cgx_attention_paged_ws": (SZ, [PPAGED, PSTEP, I]),
+    "cgx_attention_paged_dev": (I, [PPAGED, I, PSTEP, VP, I, VP, VP, VP, VP, VP, SZ]),
+    "cgx_token_logprobs_ws": (SZ, [I, I, I]),
+    "cgx_token_logprobs_dev": (I, [VP, SZ, I, I, VP, I, VP, VP, VP, VP, VP, VP, SZ]),
     # synthetic decoder and the speculative loop
     "cgx_model_new": (VP, [C.POINTER(CgxModelConfig), C.c_uint64, VP]),
     "cgx_model_free": (None, [VP]),

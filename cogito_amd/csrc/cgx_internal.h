@@ -267,6 +267,25 @@ int cgk_attn_prompt_refused(void);
 int cgk_attn_combine(const float* part_o, const float* part_ml, int splits, int nrow, int D,
                      int Nq, int H, float* O, float* lse);
 
+/* Paged cache and serving steps (paged.hip, paged_attn.hip); arguments
+ * checked by host/paged.c. */
+int cgk_paged_plan(const cgx_paged_step* s, int page_size, int num_pages, int* free_pages,
+                   const int* free_count, int* free_left);
+int cgk_paged_append(const cgx_kv_paged_int4* c, int layer, const cgx_paged_step* s,
+                     const float* qkv, int ldq, int H, const float* rope, int rope_rows,
+                     float* q_out);
+int cgk_paged_gather(const cgx_kv_paged_int4* c, int layer, const int* slots, int n, float* k,
+                     float* v);
+size_t cgk_paged_attention_ws(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H);
+int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer, const cgx_paged_step* s,
+                        const float* Q, int H, const unsigned long long* anc,
+                        const int* tree_len, float* O, float* lse, void* ws);
+/* Token log probabilities (logprobs.hip). */
+size_t cgk_logprobs_ws(int rows, int V, int n_top);
+int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens, int n_top,
+                 float* logprob, int* rank, float* entropy, int* top_tokens,
+                 float* top_logprobs, void* ws);
+
 /* Rows of a tree forward (cgx_model_forward_tree): row i sits at cache slot
  * len + i and rotary position len + rel[i]; the last tw cached keys are the
  * tree's nodes, visible to row i through anc[i]. */

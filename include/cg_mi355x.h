@@ -320,6 +320,129 @@ int cgx_attention_int4_kv_batch_dev(const float* Q, int B, int Nq, int H,
                                     int mask_kind, const unsigned long long* anc, int tw,
                                     float* O);
 
+/* -------------------------------- paged INT4 KV cache and serving steps */
+/* A KV cache in pages of page_size positions that any number of sequences
+ * share (no counterpart in the reference, whose cache holds one sequence).
+ * All four arrays live in HBM; values and scales are those of
+ * cg_kv_cache_int4 (codes [-8, 7], scale = absmax / 7 per group), laid out
+ * per layer for the attention's lanes:
+ *   k_pages  [page][head][position][D/2] bytes, dims 2i, 2i + 1 in byte i
+ *            (low nibble first);
+ *   v_pages  [page][head][position / 16][16][position % 16][D/32] bytes:
+ *            block n holds dims n D/16 .. (n + 1) D/16 - 1 of 16 positions;
+ *   scales   [page][head][position][D/group_size] fp32.
+ * page_size: a power of two, 16 to 4096; head_dim: a multiple of 32, at most
+ * 256; group_size: even, divides head_dim; num_pages * page_size below 2^31.
+ * A program may fill the struct over memory of its own (16-byte aligned)
+ * instead of taking one from cgx_kv_paged_int4_new, whose pages start zero. */
+typedef struct {
+    uint8_t* k_pages;
+    uint8_t* v_pages;
+    float* k_scales;
+    float* v_scales;
+    int num_layers;
+    int num_pages;
+    int page_size;
+    int n_heads;
+    int head_dim;
+    int group_size;
+} cgx_kv_paged_int4;
+cgx_kv_paged_int4* cgx_kv_paged_int4_new(int num_layers, int num_pages, int page_size,
+                                         int n_heads, int head_dim, int group_size);
+void cgx_kv_paged_int4_free(cgx_kv_paged_int4* cache);
+
+/* One step over a batch of sequences of different lengths: device arrays
+ * that the caller owns.  cgx_paged_plan_dev fills the second half from the
+ * first; the append and the attention read the second half only (a caller may
+ * fill it by other means). */
+typedef struct {
+    int seqs;             /* sequences, at most 4096 */
+    int rows;             /* entries of the row arrays */
+    int max_rows;         /* most rows of one sequence (0: any number) */
+    int table_ld;         /* entries of a table row */
+    const int* kv_old;    /* [seqs] positions whose pages table_old holds */
+    const int* kv_keep;   /* [seqs] of those, the positions that stay (NULL: all) */
+    const int* rows_new;  /* [seqs] rows that the step adds */
+    const int* table_old; /* [seqs][table_ld], or NULL: `table`, updated in place */
+    int* table;           /* [seqs][table_ld] page of positions e * page_size .. */
+    int* row_begin;       /* [seqs + 1] first row of each sequence */
+    int* row_seq;         /* [rows] sequence (-1 past the last row) */
+    int* row_pos;         /* [rows] position in the sequence (-1) */
+    int* row_slot;        /* [rows] page * page_size + position % page_size (-1) */
+    int* kv_len;          /* [seqs] positions after the step */
+    int* status;          /* [4] refusal bits, rows, pages taken, pages given back */
+} cgx_paged_step;
+
+/* Tables of a step, in one launch and with no word from the host: sequence b
+ * keeps kv_keep[b] of its kv_old[b] positions and adds rows_new[b] rows.  A
+ * page past the last position goes back on the stack free_pages[0 ..
+ * *free_count), sequence by sequence; then new pages are taken from its top
+ * down, sequence by sequence.  *free_left receives the new count (a word of
+ * its own, so that a step can be planned again); entries of the stack below
+ * *free_count are not written, the stack holds num_pages entries.  Table
+ * entries past a sequence's pages are left as they were in place, -1 in
+ * another table.  A sequence that ends keeps 0 and adds 0.
+ * All or nothing: with a bad length (bit 1: below 0, keep above old), a
+ * sequence of more than table_ld pages (2), more rows than `rows`, or than
+ * max_rows for one sequence (4), too few pages (8) or a stack count outside
+ * its array (16), status[0] holds those bits, row_begin is all 0, kv_len =
+ * kv_old, *free_left = *free_count, and the step has no rows.  Outputs must
+ * not overlap inputs (table_old = table excepted). */
+int cgx_paged_plan_dev(const cgx_paged_step* step, int page_size, int num_pages,
+                       int* free_pages, const int* free_count, int* free_left);
+
+/* The new rows of a step into their slots of `layer`: row t of qkv (ldq
+ * values apart) holds H query heads, then the cache's heads of K, then of V.
+ * Queries and keys are rotated (rotate-half, cg_apply_rope's operations) with
+ * the (cos, sin) of row_pos[t] in rope [rope_rows][head_dim / 2][2]
+ * (cgx_rope_table_dev from position 0; NULL: no rotation), queries stored to
+ * q_out [rows][H][head_dim] (NULL: not stored), keys and values quantised by
+ * cg_kv_cache_int4_append's rule, bit for bit.  Rows with a slot outside the
+ * cache, or a position outside rope, are skipped; two rows of one slot leave
+ * either's values. */
+int cgx_kv_paged_append_dev(cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
+                            const float* qkv, int ldq, int H, const float* rope, int rope_rows,
+                            float* q_out);
+/* The cached values of n slots: k, v [n][n_heads][head_dim] (0 for a slot
+ * outside the cache). */
+int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int* slots, int n,
+                            float* k, float* v);
+
+/* Attention of a step's rows over their sequences' pages of `layer`: Q, O
+ * [rows][H][head_dim], H a multiple of the cache's heads, scale
+ * 1/sqrt(head_dim), lse [rows][H] (natural logarithm; NULL: none).  Row i of
+ * sequence b sees keys up to kv_len[b] - (rows of b) + i; with anc (device,
+ * [rows] ancestor bits), every key below kv_len[b] - w and those keys
+ * kv_len[b] - w + j, j < w, whose bit j is set, w = tree_len[b] (at most 64;
+ * tree_len NULL: the rows of b).  A row that sees nothing gets 0 (lse -inf).
+ * Keys of a table entry outside the cache are not seen.  Rows past the last
+ * sequence's are left as they were.  Of the step: seqs, rows, max_rows,
+ * table_ld, table, row_begin, row_seq and kv_len are read; a sequence of more
+ * rows than max_rows (where given) may be left out.
+ * ws: cgx_attention_paged_ws bytes of device memory (16-byte aligned), for
+ * this call alone while it runs; every call on the library stream may use
+ * the same.  Nothing is allocated: the call may be captured into a graph. */
+size_t cgx_attention_paged_ws(const cgx_kv_paged_int4* cache, const cgx_paged_step* step, int H);
+int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
+                            const float* Q, int H, const unsigned long long* anc,
+                            const int* tree_len, float* O, float* lse, void* ws, size_t ws_bytes);
+
+/* Log probabilities of rows of logits x [rows][V] (ld floats apart), device
+ * pointers throughout.  For the given token of each row (tokens [rows], NULL:
+ * none): logprob = x[tok] - log sum exp(x) and rank, the number of tokens
+ * before it in the order (value descending, index ascending; NaN last); a
+ * token outside [0, V) has -inf and rank V.  entropy: -sum p log p, a token of
+ * probability 0 adding 0.  top_tokens, top_logprobs [rows][n_top]: the first
+ * n_top (at most 32) of that order, past V -1 and -inf.  A row that holds a
+ * NaN or +inf, or nothing above -inf, has NaN for every log probability
+ * within V and for its entropy.  NULL outputs are left out (top_tokens and
+ * top_logprobs go together).  ws: cgx_token_logprobs_ws bytes of device memory
+ * (16-byte aligned), as for cgx_attention_paged_dev. */
+size_t cgx_token_logprobs_ws(int rows, int V, int n_top);
+int cgx_token_logprobs_dev(const float* logits, size_t ld, int rows, int V, const int* tokens,
+                           int n_top, float* logprob, int* rank, float* entropy,
+                           int* top_tokens, float* top_logprobs, void* ws, size_t ws_bytes);
+
 /* ------------------------------------------------- synthetic decoder */
 /* Decoder-only transformer with INT4 weights resident in HBM, the model the
  * verify stack runs (reference src/layers/transformer.c:26-149 block order,
