@@ -5,7 +5,11 @@
 // keys: running maximum m, running sum l and O, both held relative to m.
 //
 // Lengths, row offsets and tables are device words.  Every address formed from
-// them is bounded here: a length by the table row, a page by the pool.
+// them is bounded here: a length by the table row, a page by the pool, a row
+// by the row arrays.
+//
+// Head dimensions of 32 to 128 with scales per 32 dimensions or more run on
+// the matrix cores (k_attn_paged); the rest takes k_attn_paged_row.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -14,6 +18,13 @@
 #include "cgx_internal.h"
 
 namespace {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 inline hipStream_t stream() { return (hipStream_t)cgx_stream(); }
 
@@ -43,6 +54,13 @@ struct PagedArgs {
     float scale;
     float* O;
     float* lse;
+    // k_attn_paged: sequences of r_lo .. r_hi query rows times heads a KV
+    // head, key chunks of at least c_min, about `target` units; partial
+    // results of split tiles and what k_paged_join needs of each sequence
+    int r_lo, r_hi, c_min, target, max_parts;
+    float* part_o;               // [parts][tile rows][D]
+    float* part_ml;              // [parts][tile rows][2]
+    int4* info;                  // [seqs] splits, first part, tiles, tile rows
 };
 
 __device__ __forceinline__ float code(unsigned n) { return (float)((int)(n << 28) >> 28); }
@@ -137,31 +155,742 @@ __global__ __launch_bounds__(64) void k_attn_paged_row(PagedArgs a) {
     if (a.lse && lane == 0) a.lse[(size_t)t * a.H + h] = l != 0.0f ? m + logf(l) : -INFINITY;
 }
 
+// ------------------------------------------------------- matrix-core kernel
+//
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16.  The codes of K
+// and V are exact fp16 integers.  Q (times scale log2 e) and the weights P v_s
+// (v_s the key's V scale) are each two fp16 terms, hi + lo, of a value brought
+// into [2^14, 2^15) by its row's power of two: 22 bits of it, and of values
+// down to 2^-16 of the row's largest; products are exact, sums fp32.  The K
+// scale multiplies the key's fp32 score.  A lane of group g (lane / 16) holds
+// query row lane % 16 and the scores of keys 4g .. 4g + 3 of each half tile,
+// which is the B operand of the second product, so P never moves.  Row state
+// (m, l and the exponent e of the weights) is a lane's own; the maximum goes
+// over the four lane groups with two lane-row swaps.
+//
+// The exponent follows the weights' largest of the tile, or what the sums so
+// far still need (e minus the whole part of the maximum's rise): V scales may
+// lie any distance apart.
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTile = 32;                        // keys of a wave's step
+
+__device__ __forceinline__ float max_rows(float v) {     // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float sum_rows(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// (w & mask) | 0x6400: 1024 plus the nibble (or 16 times it) in each half.
+__device__ __forceinline__ f16x2 low_nibbles(uint32_t w) {
+    const f16x2 m = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u) + m;
+}
+__device__ __forceinline__ f16x2 high_nibbles(uint32_t w) {
+    const f16x2 s = {(_Float16)0.0625f, (_Float16)0.0625f}, m = {(_Float16)-72.0f, (_Float16)-72.0f};
+    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x64006400u), s, m);
+}
+
+// Eight offset-binary codes of a word: element p is nibble slot_of(p).
+__device__ __forceinline__ int slot_of(int p) { return (p >> 1) + 4 * (p & 1); }
+__device__ __forceinline__ f16x8 codes8(uint32_t w) {
+    const f16x2 a = low_nibbles(w), b = high_nibbles(w), c = low_nibbles(w >> 8), d = high_nibbles(w >> 8);
+    f16x8 r;
+    r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
+    r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const u32x4 v = *(const u32x4*)p;
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const u32x2 v = *(const u32x2*)p;
+        w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = ((const uint32_t*)p)[i];
+    }
+}
+
+struct Unit {
+    int b, hk, tile, split, nsplit, part, L, n, r0;
+};
+
+// The block's unit of work: sequences of r_lo .. r_hi rows in order, each with
+// Hk * tiles * nsplit units.  The chunk length C follows from the keys of all
+// of them, so that there are about `target` units whatever the lengths; a
+// sequence is cut into round(len / C) even pieces.  Every block finds this out
+// for itself from the lengths: a few hundred words, against a launch more and
+// a wait for it.
+template <int TROWS>
+__device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
+    __shared__ long long s_sum[3][kWaves];
+    __shared__ Unit s_unit;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = a.seqs, G = a.H / a.Hk;
+    const long long most = (long long)a.table_ld << a.lp;
+    struct Seq { int r0, n, L, tiles; };
+    auto seq = [&](int b) {
+        Seq s;
+        s.r0 = min(max(a.row_begin[b], 0), a.rows);
+        s.n = max(0, min(a.row_begin[b + 1], a.rows) - s.r0);
+        s.L = (int)min((long long)max(a.kv_len[b], 0), most);
+        const long long R = (long long)s.n * G;
+        s.tiles = R >= a.r_lo && R <= a.r_hi ? (int)((R + TROWS - 1) / TROWS) : 0;
+        return s;
+    };
+    if (tid == 0) s_unit.b = -1;
+    const int per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    long long work = 0;
+    for (int b = b0; b < b1; b++) {
+        const Seq s = seq(b);
+        work += (long long)s.tiles * s.L;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
+    if (lane == 0) s_sum[2][wave] = work;
+    __syncthreads();
+    work = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) work += s_sum[2][w];
+    long long C = (work * a.Hk + a.target - 1) / a.target;
+    C = (max(C, (long long)a.c_min) + kTile - 1) / kTile * kTile;
+    auto splits = [&](const Seq& s) {
+        return max(1, (int)((s.L + C / 2) / C));
+    };
+    long long units = 0, parts = 0;
+    for (int b = b0; b < b1; b++) {
+        const Seq s = seq(b);
+        const int ns = splits(s);
+        units += (long long)s.tiles * a.Hk * ns;
+        if (ns > 1) parts += (long long)s.tiles * a.Hk * ns;
+    }
+    long long iu = units, ip = parts;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long x = __shfl_up(iu, o), y = __shfl_up(ip, o);
+        if (lane >= o) {
+            iu += x;
+            ip += y;
+        }
+    }
+    if (lane == 63) {
+        s_sum[0][wave] = iu;
+        s_sum[1][wave] = ip;
+    }
+    __syncthreads();
+    long long pu = iu - units, pp = ip - parts;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++)
+        if (w < wave) {
+            pu += s_sum[0][w];
+            pp += s_sum[1][w];
+        }
+    const long long me = blockIdx.x;
+    if (me >= pu && me < pu + units) {
+        for (int b = b0; b < b1; b++) {
+            const Seq s = seq(b);
+            const int ns = splits(s);
+            const long long here = (long long)s.tiles * a.Hk * ns;
+            if (me < pu + here) {
+                // KV heads fastest: with 8 of them a head's pieces share an XCD's L2
+                const int x = (int)(me - pu), y = x / a.Hk;
+                Unit f;
+                f.b = b;
+                f.hk = x % a.Hk;
+                f.tile = y % s.tiles;
+                f.split = y / s.tiles;
+                f.nsplit = ns;
+                f.L = s.L;
+                f.n = s.n;
+                f.r0 = s.r0;
+                const long long first = pp;
+                f.part = -1;
+                if (ns > 1) {
+                    const long long at = first + ((long long)f.hk * s.tiles + f.tile) * ns + f.split;
+                    f.part = at < a.max_parts ? (int)at : -2;
+                }
+                if (x == 0)
+                    a.info[b] = make_int4(ns, (int)min(first, (long long)a.max_parts), s.tiles, TROWS);
+                s_unit = f;
+                break;
+            }
+            pu += here;
+            if (ns > 1) pp += here;
+        }
+    }
+    __syncthreads();
+    u = s_unit;
+    // the same in every lane: scalars
+    u.b = __builtin_amdgcn_readfirstlane(u.b);
+    u.hk = __builtin_amdgcn_readfirstlane(u.hk);
+    u.tile = __builtin_amdgcn_readfirstlane(u.tile);
+    u.split = __builtin_amdgcn_readfirstlane(u.split);
+    u.nsplit = __builtin_amdgcn_readfirstlane(u.nsplit);
+    u.part = __builtin_amdgcn_readfirstlane(u.part);
+    u.L = __builtin_amdgcn_readfirstlane(u.L);
+    u.n = __builtin_amdgcn_readfirstlane(u.n);
+    u.r0 = __builtin_amdgcn_readfirstlane(u.r0);
+    return u.b >= 0;
+}
+
+// One unit.  NC = D / 32, NG scales a head row, RT tiles of 16 query rows a
+// wave; KS: the block's waves share the rows and take the tiles of 32 keys in
+// turn (few rows, the sums joined in LDS), else each wave has rows of its own
+// over all of the unit's keys.
+template <int NC, int NG, int RT, bool KS>
+__global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
+    constexpr int D = 32 * NC, half = D / 2, TROWS = 16 * RT * (KS ? 1 : kWaves);
+    constexpr int GD = D / NG, TPG = GD / 16, NT = D / 16;   // dims, O tiles a group; O tiles
+    constexpr int QW = KS ? 1 : kWaves;
+    __shared__ f16x8 s_q[QW][RT][NC][2][64];
+    __shared__ float s_o[KS ? kWaves / 2 : 1][KS ? 16 * RT : 1][KS ? D + 4 : 1];
+    __shared__ float s_ml[KS ? kWaves : 1][KS ? 16 * RT : 1][2];
+    Unit u;
+    if (!find_unit<TROWS>(a, u)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4, G = a.H / a.Hk, R = u.n * G, L = u.L;
+    const int row0 = u.tile * TROWS + (KS ? 0 : wave * 16 * RT);
+    const int hk = u.hk, b = u.b, lp = a.lp, pmask = (1 << lp) - 1;
+
+    // chain: keys up to base + i; tree: keys below base and those of the bits
+    int base = L - u.n;
+    if (a.anc && a.tree_len) base = L - min(max(a.tree_len[b], 0), L);
+    if (a.anc) base = max(base, 0);
+    int rq[RT];                                  // the row's entry of the row arrays
+    bool rok[RT];
+    int lim[RT];                                 // last key seen without a bit
+    unsigned long long bits[RT];
+    size_t qrow[RT];
+    int end = 0;                                 // keys that any of the wave's rows may see
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int r = row0 + 16 * rt + n;
+        rok[rt] = r < R;
+        const int i = rok[rt] ? r / G : 0, h = hk * G + (rok[rt] ? r - i * G : 0);
+        rq[rt] = u.r0 + i;
+        qrow[rt] = (size_t)rq[rt] * a.H + h;
+        lim[rt] = !rok[rt] ? -1 : a.anc ? base - 1 : base + i;
+        bits[rt] = a.anc && rok[rt] ? a.anc[rq[rt]] : 0;
+        const int last = min(R - 1, row0 + 16 * rt + 15);
+        if (row0 + 16 * rt < R) end = max(end, a.anc ? L : min(L, base + last / G + 1));
+    }
+    // the unit's piece of the keys, and what all of the wave's rows see of it
+    const int piece = ((L + u.nsplit - 1) / u.nsplit + kTile - 1) / kTile * kTile;
+    const int k_begin = u.split * piece;
+    end = min(end, min(L, k_begin + piece));
+    const int first_i = row0 < R ? row0 / G : 0;
+    const int open_end = row0 < R ? min(L, a.anc ? base : base + first_i + 1) : 0;
+
+    // ---- Q^T operands: element p of chunk c is dim (NG == 1) g D/4 + 8 c +
+    //      slot, (NG > 1) 32 c + 8 g + slot, so that a product never spans
+    //      two scale groups
+    float qinv[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float* q = a.Q + qrow[rt] * D;
+        float v[NC][8], top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int x = 0; x < 8; x += 4) {
+                const float4 t = *(const float4*)(q + (NG == 1 ? g * (D / 4) + 8 * c : 32 * c + 8 * g) + x);
+                v[c][x] = t.x; v[c][x + 1] = t.y; v[c][x + 2] = t.z; v[c][x + 3] = t.w;
+            }
+        const float f = a.scale * 1.44269504088896340736f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                v[c][x] = rok[rt] ? v[c][x] * f : 0.0f;
+                top = fmaxf(top, fabsf(v[c][x]));
+            }
+        top = max_rows(top);
+        // 2^e <= top < 2^(e + 1); far exponents are cut where fp16's range covers them
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = min(max(e, -100), 127);
+        qinv[rt] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+        const int up = 14 - e;
+        if (KS && wave != rt) continue;          // shared rows: one writer
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            f16x8 hi, lo;
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                const float x = ldexpf(v[c][slot_of(p)], up);
+                hi[p] = (_Float16)x;
+                lo[p] = (_Float16)(x - (float)hi[p]);
+            }
+            s_q[KS ? 0 : wave][rt][c][0][lane] = hi;
+            s_q[KS ? 0 : wave][rt][c][1][lane] = lo;
+        }
+    }
+    __syncthreads();
+
+    // ---- V^T operands: group y's O tile t has dims y GD + TPG n + t of lane
+    //      n, that is bytes beta .. of block blk of the V page
+    int voff[NG], beta[NG];
+#pragma unroll
+    for (int y = 0; y < NG; y++) {
+        const int d0 = y * GD + n * TPG;
+        voff[y] = (d0 / (2 * NC)) * (16 * NC) + 4 * g * NC;
+        beta[y] = NG == 1 ? 0 : d0 % (2 * NC) / 2;
+    }
+    struct Tile {
+        uint32_t k[2][NC], v[2][NG][NC];
+        f32x4 ks[2][NG], vs[2][NG];
+        int ok;                                  // bit h: half h's page is in the pool
+    };
+    const int* tab = a.table + (size_t)b * a.table_ld;
+    struct Pages { int p[2]; };
+    auto pages = [&](int kt) {
+        Pages x;
+#pragma unroll
+        for (int h = 0; h < 2; h++) x.p[h] = kt + 16 * h < end ? tab[(kt + 16 * h) >> lp] : -1;
+        return x;
+    };
+    auto load = [&](int kt, const Pages& pg, Tile& t) {
+        t.ok = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const bool in = pg.p[h] >= 0 && pg.p[h] < a.num_pages;
+            t.ok |= in << h;
+            const size_t row = (((size_t)(in ? pg.p[h] : 0) * a.Hk + hk) << lp) + ((kt + 16 * h) & pmask);
+            const uint8_t* kp = a.kp + row * half;
+            if constexpr (NG == 1) {
+                load_words<NC>(kp + (uint32_t)(n * half + 4 * NC * g), t.k[h]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++) t.k[h][c] = *(const uint32_t*)(kp + (uint32_t)(n * half + 16 * c + 4 * g));
+            }
+            const float* sp = a.ks + row * NG;
+#pragma unroll
+            for (int y = 0; y < NG; y++) t.ks[h][y] = *(const f32x4*)(sp + (uint32_t)(4 * g * NG + 4 * y));
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const bool in = (t.ok >> h) & 1;
+            const size_t row = (((size_t)(in ? pg.p[h] : 0) * a.Hk + hk) << lp) + ((kt + 16 * h) & pmask);
+            const uint8_t* vp = a.vp + row * half;       // 16 positions of a head: 16 half bytes
+#pragma unroll
+            for (int y = 0; y < NG; y++) load_words<NC>(vp + (uint32_t)voff[y], t.v[h][y]);
+            const float* sp = a.vs + row * NG;
+#pragma unroll
+            for (int y = 0; y < NG; y++) t.vs[h][y] = *(const f32x4*)(sp + (uint32_t)(4 * g * NG + 4 * y));
+        }
+    };
+
+    float m[RT], l[RT];
+    int ew[RT][NG];
+    f32x4 o[RT][NT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int y = 0; y < NG; y++) ew[rt][y] = -100;
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[rt][t] = (f32x4)(0.0f);
+    }
+
+    auto process = [&](const Tile& td, int kt) {
+        int ql = lane;
+        asm volatile("" : "+v"(ql));             // Q is read again each tile, not kept in registers
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f32x4 acc[RT];
+#pragma unroll
+            for (int y = 0; y < NG; y++) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) acc[rt] = (f32x4)(0.0f);
+#pragma unroll
+                for (int c = y * NC / NG; c < (y + 1) * NC / NG; c++) {
+                    const f16x8 kc = codes8(td.k[h][c] ^ 0x88888888u);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[KS ? 0 : wave][rt][c][0][ql], acc[rt], 0, 0, 0);
+                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[KS ? 0 : wave][rt][c][1][ql], acc[rt], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        // scales of key x: [x * NG + y] of the four keys' scales
+                        const float sc = td.ks[h][(x * NG + y) / 4][(x * NG + y) % 4];
+                        s[rt][h][x] = y ? s[rt][h][x] + acc[rt][x] * sc : acc[rt][x] * sc;
+                    }
+            }
+        }
+        const bool open = td.ok == 3 && kt + kTile <= open_end && kt + kTile <= end;
+        unsigned see[RT];
+        float drop[RT], pr[RT][8];
+        int whole[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            see[rt] = 0xffu;
+            if (!open) {
+                see[rt] = 0;
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    const int key = kt + (p < 4 ? 4 * g + p : 12 + 4 * g + p), d = key - base;
+                    const bool bit = key >= base && d < 64 && ((bits[rt] >> (d & 63)) & 1);
+                    const bool yes = key < end && ((td.ok >> (p >> 2)) & 1) && (key <= lim[rt] || bit);
+                    see[rt] |= (unsigned)yes << p;
+                    s[rt][p >> 2][p & 3] = yes ? s[rt][p >> 2][p & 3] : -INFINITY;
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < 8; p++) top = fmaxf(top, s[rt][p >> 2][p & 3]);
+            const float mn = fmaxf(m[rt], max_rows(top) * qinv[rt]);
+            // a score that is NaN leaves m alone and makes l NaN; without any
+            // score so far every weight is exp2(-inf) = 0
+            const float mu = mn == -INFINITY ? 0.0f : mn;
+            drop[rt] = m[rt] == mn ? 0.0f : mn - m[rt];
+            m[rt] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                pr[rt][p] = __builtin_amdgcn_exp2f(fmaf(s[rt][p >> 2][p & 3], qinv[rt], -mu));
+                sum += pr[rt][p];
+            }
+            l[rt] = l[rt] * __builtin_amdgcn_exp2f(-drop[rt]) + sum;
+            whole[rt] = (int)fminf(drop[rt], 300.0f);
+        }
+#pragma unroll
+        for (int y = 0; y < NG; y++) {
+            f16x8 hi[RT], lo[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                float w[8], big = 0.0f;
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    const int e = (p & 3) * NG + y;
+                    const float vs = td.vs[p >> 2][e / 4][e % 4];
+                    // a hidden key's scale may be anything
+                    w[p] = open || ((see[rt] >> p) & 1) ? pr[rt][p] * vs : 0.0f;
+                    big = fmaxf(big, fabsf(w[p]));
+                }
+                big = max_rows(big);
+                const int et = (int)(__float_as_uint(big) >> 23) - 127;
+                const int en = max(max(et, ew[rt][y] - whole[rt]), -100);
+                const float f = __builtin_amdgcn_exp2f((float)(ew[rt][y] - en) - drop[rt]);
+                ew[rt][y] = en;
+                const float up = __uint_as_float((uint32_t)(14 - en + 127) << 23);
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    const float x = w[p] * up;
+                    hi[rt][p] = (_Float16)x;
+                    lo[rt][p] = (_Float16)(x - (float)hi[rt][p]);
+                }
+                if (__any(f != 1.0f)) {
+#pragma unroll
+                    for (int t = 0; t < TPG; t++) o[rt][y * TPG + t] *= f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TPG; t++) {
+                const uint32_t at = (uint32_t)(beta[y] + t / 2) * 0x10001u;
+                constexpr int b23 = NC == 4 ? 2 : NC == 1 ? 0 : 1;         // first word of keys 2, 3
+                const uint32_t s01 = (0x0C000C00u | (NC << 16)) + at;
+                const uint32_t s23 = (0x0C000C00u | ((3 * NC - 4 * b23) << 16) | (2 * NC - 4 * b23)) + at;
+                f16x8 va;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t (&v)[NC] = td.v[h][y];
+                    const uint32_t w01 = __builtin_amdgcn_perm(v[NC > 2 ? 1 : 0], v[0], s01) ^ 0x00880088u;
+                    const uint32_t w23 = __builtin_amdgcn_perm(v[NC > 2 ? b23 + 1 : b23], v[b23], s23) ^ 0x00880088u;
+                    const f16x2 x = t & 1 ? high_nibbles(w01) : low_nibbles(w01);
+                    const f16x2 z = t & 1 ? high_nibbles(w23) : low_nibbles(w23);
+                    va[4 * h] = x[0]; va[4 * h + 1] = x[1]; va[4 * h + 2] = z[0]; va[4 * h + 3] = z[1];
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    o[rt][y * TPG + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, hi[rt], o[rt][y * TPG + t], 0, 0, 0);
+                    o[rt][y * TPG + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, lo[rt], o[rt][y * TPG + t], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    constexpr int step = KS ? kWaves * kTile : kTile;
+    int kt = k_begin + (KS ? wave * kTile : 0);
+    if constexpr (NG == 1) {
+        if (kt < end) {
+            Tile cur, nxt;
+            load(kt, pages(kt), cur);
+            Pages ahead = pages(kt + step);
+            for (;;) {
+                const int next = kt + step;
+                if (next >= end) break;
+                load(next, ahead, nxt);
+                ahead = pages(next + step);
+                process(cur, kt);
+                cur = nxt;
+                kt = next;
+            }
+            process(cur, kt);
+        }
+    } else {
+        // the scales and words of several groups leave no registers for a
+        // second tile
+        Pages ahead = pages(kt);
+        for (; kt < end; kt += step) {
+            Tile cur;
+            load(kt, ahead, cur);
+            ahead = pages(kt + step);
+            process(cur, kt);
+        }
+    }
+
+    // ---- row sums, and O back to one scale relative to m
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        l[rt] = sum_rows(l[rt]);
+#pragma unroll
+        for (int y = 0; y < NG; y++) {
+            const float dn = __uint_as_float((uint32_t)(ew[rt][y] - 14 + 127) << 23);
+#pragma unroll
+            for (int t = 0; t < TPG; t++) o[rt][y * TPG + t] *= dn;
+        }
+    }
+    // element x of a group's O tiles is TPG neighbouring dims of lane group g
+    auto dim = [&](int y, int x) { return y * GD + (4 * g + x) * TPG; };
+    auto put = [&](float* to, const f32x4 (&v)[NT], float f) {
+#pragma unroll
+        for (int y = 0; y < NG; y++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int t = 0; t < TPG; t += 2)
+                    *(f32x2*)(to + dim(y, x) + t) = (f32x2){v[y * TPG + t][x] * f, v[y * TPG + t + 1][x] * f};
+    };
+
+    if constexpr (KS) {
+        // the waves' maxima and sums, then O of waves 2, 3 onto 0, 1, and 1 onto 0
+        if (g == 0) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                s_ml[wave][16 * rt + n][0] = m[rt];
+                s_ml[wave][16 * rt + n][1] = l[rt];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) M = fmaxf(M, s_ml[w][16 * rt + n][0]);
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float mw = s_ml[w][16 * rt + n][0];
+                sum += s_ml[w][16 * rt + n][1] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+            }
+            const float f = m[rt] == M ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - M);
+            m[rt] = M;
+            l[rt] = sum;
+#pragma unroll
+            for (int t = 0; t < NT; t++) o[rt][t] *= f;
+        }
+#pragma unroll
+        for (int from = kWaves / 2; from > 0; from >>= 1) {
+            if (wave >= from && wave < 2 * from) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) put(&s_o[wave - from][16 * rt + n][0], o[rt], 1.0f);
+            }
+            __syncthreads();
+            if (wave < from) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int y = 0; y < NG; y++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll
+                            for (int t = 0; t < TPG; t++) o[rt][y * TPG + t][x] += s_o[wave][16 * rt + n][dim(y, x) + t];
+            }
+            __syncthreads();
+        }
+        if (wave != 0) return;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (!rok[rt] || u.part == -2) continue;
+        if (u.part < 0) {
+            const float inv = l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f;
+            put(a.O + qrow[rt] * D, o[rt], inv);
+            if (a.lse && g == 0)
+                a.lse[qrow[rt]] = l[rt] != 0.0f ? 0.69314718055994530942f * (m[rt] + log2f(l[rt])) : -INFINITY;
+        } else {
+            const size_t pr = (size_t)u.part * TROWS + (row0 - u.tile * TROWS) + 16 * rt + n;
+            put(a.part_o + pr * D, o[rt], 1.0f);
+            if (g == 0) {
+                a.part_ml[2 * pr] = m[rt];
+                a.part_ml[2 * pr + 1] = l[rt];
+            }
+        }
+    }
+}
+
+// Joins the pieces of split rows: block = (row, head), its waves take pieces
+// in turn; m relative to the largest of the pieces, as in the block itself.
+__global__ __launch_bounds__(kThreads) void k_paged_join(PagedArgs a) {
+    __shared__ float s_o[kWaves][128], s_l[kWaves], s_m[kWaves];
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = a.row_seq[t];
+    if (b < 0 || b >= a.seqs) return;
+    const int r0 = min(max(a.row_begin[b], 0), a.rows), i = t - r0;
+    const int n = max(0, min(a.row_begin[b + 1], a.rows) - r0), G = a.H / a.Hk;
+    if (i < 0 || i >= n || (long long)n * G < a.r_lo || (long long)n * G > a.r_hi) return;
+    const int4 f = a.info[b];
+    const int ns = f.x, tiles = f.z, trows = f.w;
+    if (ns < 2) return;
+    const int hk = h / G, r = i * G + (h - hk * G), tile = r / trows;
+    const long long at = f.y + ((long long)hk * tiles + tile) * ns;
+    if (tile >= tiles || at + ns > a.max_parts) return;
+    const size_t p0 = (size_t)at * trows + (r - tile * trows);
+    const int D = a.D;
+    float M = -INFINITY;
+    for (int s = lane; s < ns; s += 64) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * trows)]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    const int d = 2 * lane;
+    for (int s = wave; s < ns; s += kWaves) {
+        const size_t p = p0 + (size_t)s * trows;
+        const float mw = a.part_ml[2 * p], w = mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M);
+        l += w * a.part_ml[2 * p + 1];
+        if (d < D) {
+            const f32x2 v = *(const f32x2*)(a.part_o + p * D + d);
+            o0 += w * v.x;
+            o1 += w * v.y;
+        }
+    }
+    if (d < D) {
+        s_o[wave][d] = o0;
+        s_o[wave][d + 1] = o1;
+    }
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) l += s_l[w];
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    for (int x = threadIdx.x; x < D; x += kThreads) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) v += s_o[w][x];
+        a.O[((size_t)t * a.H + h) * D + x] = v * inv;
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[(size_t)t * a.H + h] = l != 0.0f ? 0.69314718055994530942f * (M + log2f(l)) : -INFINITY;
+}
+
 int log2i(int x) {
     int l = 0;
     while ((1 << l) < x) l++;
     return l;
 }
 
+// How a call is cut: the split launch (few rows a KV head, keys over the
+// waves) and the tile launch (more rows, rows over the waves).
+struct Launch {
+    int rt, r_lo, r_hi, c_min, target, max_parts;
+    long long grid;
+    size_t part_o, part_ml;      // bytes
+};
+struct Plan {
+    bool fast;
+    Launch l[2];
+    int n;
+    size_t info, total;
+};
+
+constexpr int kSplitRows = 32;
+
+Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
+    Plan p = {};
+    const int D = c->head_dim, G = H / c->n_heads;
+    p.fast = D <= 128 && c->group_size % 32 == 0;
+    if (!p.fast || !s->rows) return p;
+    const long long most = s->max_rows && s->max_rows < s->rows ? s->max_rows : s->rows;
+    const long long R = most * G, seqs = s->seqs < s->rows ? s->seqs : s->rows;
+    const long long keys = (long long)s->table_ld * c->page_size;
+    auto add = [&](int rt, bool ks, int lo, long long hi, long long tiles, int c_min, int target) {
+        Launch& l = p.l[p.n++];
+        const int trows = 16 * rt * (ks ? 1 : kWaves);
+        l.rt = ks ? rt : -rt;
+        l.r_lo = lo;
+        l.r_hi = (int)(hi > 0x7fffffff ? 0x7fffffff : hi);
+        l.c_min = c_min;
+        l.target = target;
+        // round(len / C) pieces: at most target units by length and one a tile
+        const long long whole = tiles * c->n_heads, pieces = (keys + c_min / 2) / c_min;
+        l.grid = whole + target;
+        if (l.grid > whole * (pieces < 1 ? 1 : pieces)) l.grid = whole * (pieces < 1 ? 1 : pieces);
+        // a split tile has at least 1.5 C keys, so at most 4/3 target pieces in all
+        l.max_parts = pieces > 1 ? target * 4 / 3 + 1 : 0;
+        if (l.max_parts > l.grid) l.max_parts = (int)l.grid;
+        l.part_o = (size_t)l.max_parts * trows * D * 4;
+        l.part_ml = (size_t)l.max_parts * trows * 2 * 4;
+        p.total += l.part_o + l.part_ml;
+    };
+    p.info = (size_t)s->seqs * sizeof(int4);
+    p.total = p.info;
+    add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 1024);
+    if (R > kSplitRows)
+        add(2, false, kSplitRows + 1, 0x7fffffff, ((long long)s->rows * G) / 128 + seqs, 256, 256);
+    return p;
+}
+
+template <int NC, int NG>
+void launch_shape(const Launch& l, const PagedArgs& a) {
+    const dim3 grid((unsigned)l.grid), block(kThreads);
+    if (l.rt == 1) hipLaunchKernelGGL((k_attn_paged<NC, NG, 1, true>), grid, block, 0, stream(), a);
+    else if (l.rt == 2) hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, true>), grid, block, 0, stream(), a);
+    else hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, false>), grid, block, 0, stream(), a);
+}
+
+void launch(const Launch& l, const PagedArgs& a) {
+    const int nc = a.D / 32, ng = a.D / a.gs;
+    switch (8 * nc + ng) {
+        case 9: launch_shape<1, 1>(l, a); break;
+        case 17: launch_shape<2, 1>(l, a); break;
+        case 18: launch_shape<2, 2>(l, a); break;
+        case 25: launch_shape<3, 1>(l, a); break;
+        case 27: launch_shape<3, 3>(l, a); break;
+        case 33: launch_shape<4, 1>(l, a); break;
+        case 34: launch_shape<4, 2>(l, a); break;
+        default: launch_shape<4, 4>(l, a); break;
+    }
+}
+
 }  // namespace
 
 extern "C" size_t cgk_paged_attention_ws(const cgx_kv_paged_int4* c, const cgx_paged_step* s,
                                          int H) {
-    (void)c;
-    (void)s;
-    (void)H;
-    return 0;
+    return plan_of(c, s, H).total;
 }
 
 extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
                                    const cgx_paged_step* s, const float* Q, int H,
                                    const unsigned long long* anc, const int* tree_len, float* O,
                                    float* lse, void* ws) {
-    (void)ws;
     const size_t rows = (size_t)c->num_pages * c->page_size * c->n_heads;
     const size_t bytes = rows * (size_t)(c->head_dim / 2) * layer;
     const size_t groups = rows * (size_t)(c->head_dim / c->group_size) * layer;
-    PagedArgs a;
+    PagedArgs a = {};
     a.kp = c->k_pages + bytes;
     a.vp = c->v_pages + bytes;
     a.ks = c->k_scales + groups;
@@ -185,6 +914,34 @@ extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
     a.scale = 1.0f / sqrtf((float)c->head_dim);
     a.O = O;
     a.lse = lse;
-    hipLaunchKernelGGL(k_attn_paged_row, dim3(s->rows, H), dim3(64), 0, stream(), a);
-    return launch_check("k_attn_paged_row");
+    const Plan p = plan_of(c, s, H);
+    if (!p.fast) {
+        hipLaunchKernelGGL(k_attn_paged_row, dim3(s->rows, H), dim3(64), 0, stream(), a);
+        return launch_check("k_attn_paged_row");
+    }
+    char* w = (char*)ws;
+    a.info = (int4*)w;
+    w += p.info;
+    for (int i = 0; i < p.n; i++) {
+        const Launch& l = p.l[i];
+        if (l.grid > 0x7fffffff) {
+            cgx_set_error("cgx_attention_paged_dev: a step of too many rows for one call");
+            return -1;
+        }
+        a.r_lo = l.r_lo;
+        a.r_hi = l.r_hi;
+        a.c_min = l.c_min;
+        a.target = l.target;
+        a.max_parts = l.max_parts;
+        a.part_o = (float*)w;
+        w += l.part_o;
+        a.part_ml = (float*)w;
+        w += l.part_ml;
+        launch(l, a);
+        if (launch_check("k_attn_paged")) return -1;
+        if (!l.max_parts) continue;
+        hipLaunchKernelGGL(k_paged_join, dim3(s->rows, H), dim3(kThreads), 0, stream(), a);
+        if (launch_check("k_paged_join")) return -1;
+    }
+    return 0;
 }

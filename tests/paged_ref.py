@@ -132,7 +132,7 @@ class Batch:
             self.table[b, :need[b]] = order[at:at + need[b]]
             at += need[b]
         self.pool = Pool(layers, pages, P, Hk, D, gs)
-        self.K, self.V = [], []
+        self.K, self.V, self.vs = [], [], []
         for b in range(B):
             n = kv[b]
             k = rng.normal(size=(n, Hk, D)).astype(np.float32)
@@ -148,6 +148,7 @@ class Batch:
                 self.pool.put(layer, slot, kc[j], ks[j], vc[j], vs[j])
             self.K.append(values(kc, ks))
             self.V.append(values(vc, vs))
+            self.vs.append(vs.astype(np.float64))
         self.begin = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
         self.T = int(self.begin[-1]) + pad
         self.seq = np.full(self.T, -1, np.int32)
@@ -170,7 +171,7 @@ class Batch:
     def attend(self, anc=None, tree_len=None, lse=True, fill=7.0, max_rows=0):
         """(O, lse) of the library, both started at `fill`."""
         lib, T, H, D = self.lib, self.T, self.H, self.D
-        o = DeviceArray.from_numpy(lib, np.full((T, H, D), fill, np.float32))
+        o = DeviceArray.from_numpy(lib, np.full(T * H * D + 512, fill, np.float32))     # guard words behind
         ls = DeviceArray.from_numpy(lib, np.full((T, H), fill, np.float32)) if lse else None
         da = DeviceArray.from_numpy(lib, np.asarray(anc, np.uint64)) if anc is not None else None
         dl = DeviceArray.from_numpy(lib, np.asarray(tree_len, np.int32)) if tree_len is not None else None
@@ -185,6 +186,7 @@ class Batch:
         assert rc == 0, last_error(lib)
         assert lib.cgx_synchronize() == 0, last_error(lib)
         assert np.all(ws.numpy(np.uint8, (need + 256,))[need:] == 0xC3)
+        assert np.all(o.numpy(np.float32, (T * H * D + 512,))[T * H * D:] == fill)
         return o.numpy(np.float32, (T, H, D)), ls.numpy(np.float32, (T, H)) if lse else None
 
     def visible(self, b, anc=None, tree_len=None, seen=None):
@@ -204,9 +206,9 @@ class Batch:
         return vis
 
     def reference(self, anc=None, tree_len=None, seen=None):
-        """O, lse and A = sum_j p_j |v_j| (the scale of O's rounding errors) in 64 bits."""
+        """O, lse, A = sum_j p_j |v_j| (the scale of O's rounding errors) and N 2^-36 max_j p_j s_j, in 64 bits."""
         T, H, Hk, D = self.T, self.H, self.Hk, self.D
-        O, A, ls = np.zeros((T, H, D)), np.zeros((T, H, D)), np.full((T, H), -np.inf)
+        O, A, F, ls = np.zeros((T, H, D)), np.zeros((T, H, D)), np.zeros((T, H, D)), np.full((T, H), -np.inf)
         for b in range(len(self.kv)):
             r0, r1 = self.begin[b], self.begin[b + 1]
             if r1 == r0 or self.kv[b] == 0:
@@ -223,6 +225,8 @@ class Batch:
                 p = e / np.where(z > 0, z, 1.0)
                 O[r0:r1, h] = p @ self.V[b][:, hk]
                 A[r0:r1, h] = p @ np.abs(self.V[b][:, hk])
+                w = np.nan_to_num(p[:, :, None] * self.vs[b][None, :, hk], nan=0.0).max(1)
+                F[r0:r1, h] = np.repeat(w, self.gs, -1) * self.kv[b] * 2.0 ** -36
                 with np.errstate(divide="ignore"):
                     ls[r0:r1, h] = (m + np.log(z))[:, 0]
-        return O, ls, A
+        return O, ls, A, F
