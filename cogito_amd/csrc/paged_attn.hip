@@ -188,24 +188,54 @@ __device__ __forceinline__ float sum_rows(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// (w & mask) | 0x6400: 1024 plus the nibble (or 16 times it) in each half.
-__device__ __forceinline__ f16x2 low_nibbles(uint32_t w) {
-    const f16x2 m = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u) + m;
+// Masks in SGPRs and the fp16 exponent bits in a VGPR, made where the compiler
+// does not see constants: (w & mask) | mag is then one v_and_or_b32 (VOP3 takes
+// no literals here), else two instructions.
+struct Nib {
+    uint32_t lo, hi, mag;
+};
+__device__ __forceinline__ Nib nib_consts() {
+    Nib k;
+    asm volatile("s_mov_b32 %0, 0x000f000f" : "=s"(k.lo));
+    asm volatile("s_mov_b32 %0, 0x00f000f0" : "=s"(k.hi));
+    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(k.mag));
+    return k;
 }
-__device__ __forceinline__ f16x2 high_nibbles(uint32_t w) {
+
+// Nibbles 0 and 4 (or 1 and 5) of a word of offset-binary codes, exact: 0x6400
+// with a nibble is 1024 + n, or 1024 + 16 n.
+__device__ __forceinline__ f16x2 low_nibbles(uint32_t w, const Nib& k) {
+    const f16x2 m = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    return __builtin_bit_cast(f16x2, (w & k.lo) | k.mag) + m;
+}
+__device__ __forceinline__ f16x2 high_nibbles(uint32_t w, const Nib& k) {
     const f16x2 s = {(_Float16)0.0625f, (_Float16)0.0625f}, m = {(_Float16)-72.0f, (_Float16)-72.0f};
-    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x64006400u), s, m);
+    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & k.hi) | k.mag), s, m);
 }
 
 // Eight offset-binary codes of a word: element p is nibble slot_of(p).
 __device__ __forceinline__ int slot_of(int p) { return (p >> 1) + 4 * (p & 1); }
-__device__ __forceinline__ f16x8 codes8(uint32_t w) {
-    const f16x2 a = low_nibbles(w), b = high_nibbles(w), c = low_nibbles(w >> 8), d = high_nibbles(w >> 8);
+__device__ __forceinline__ f16x8 codes8(uint32_t w, const Nib& k) {
+    const f16x2 a = low_nibbles(w, k), b = high_nibbles(w, k), c = low_nibbles(w >> 8, k),
+                d = high_nibbles(w >> 8, k);
     f16x8 r;
     r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
     r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
     return r;
+}
+
+// x[p] * up as hi + lo, up a power of two: the product is exact, and so is
+// what hi leaves of it.
+__device__ __forceinline__ void split8(const float (&x)[8], float up, f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int p = 0; p < 8; p += 2) {
+        const f32x2 v = {x[p] * up, x[p + 1] * up};
+        const f16x2 h = __builtin_convertvector(v, f16x2);
+        const f32x2 r = {fmaf(x[p], up, -(float)h[0]), fmaf(x[p + 1], up, -(float)h[1])};
+        const f16x2 q = __builtin_convertvector(r, f16x2);
+        hi[p] = h[0]; hi[p + 1] = h[1];
+        lo[p] = q[0]; lo[p + 1] = q[1];
+    }
 }
 
 template <int N>
@@ -232,52 +262,59 @@ struct Unit {
 // sequence is cut into round(len / C) even pieces.  Every block finds this out
 // for itself from the lengths: a few hundred words, against a launch more and
 // a wait for it.
+//
+// The counts are 32 bits: consistent lengths stay below the grid, and others
+// may wrap, where a unit is only ever one that some sequence has.
 template <int TROWS>
 __device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
-    __shared__ long long s_sum[3][kWaves];
+    __shared__ float s_work[kWaves];
+    __shared__ uint32_t s_sum[2][kWaves];
     __shared__ Unit s_unit;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = a.seqs, G = a.H / a.Hk;
     const long long most = (long long)a.table_ld << a.lp;
     struct Seq { int r0, n, L, tiles; };
     auto seq = [&](int b) {
-        Seq s;
-        s.r0 = min(max(a.row_begin[b], 0), a.rows);
-        s.n = max(0, min(a.row_begin[b + 1], a.rows) - s.r0);
-        s.L = (int)min((long long)max(a.kv_len[b], 0), most);
+        Seq s = {0, 0, 0, 0};
+        if (b >= B) return s;
+        const int r0 = a.row_begin[b], r1 = a.row_begin[b + 1], kv = a.kv_len[b];
+        s.r0 = min(max(r0, 0), a.rows);
+        s.n = max(0, min(r1, a.rows) - s.r0);
+        s.L = (int)min((long long)max(kv, 0), most);
         const long long R = (long long)s.n * G;
         s.tiles = R >= a.r_lo && R <= a.r_hi ? (int)((R + TROWS - 1) / TROWS) : 0;
         return s;
     };
     if (tid == 0) s_unit.b = -1;
-    const int per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
-    long long work = 0;
-    for (int b = b0; b < b1; b++) {
-        const Seq s = seq(b);
-        work += (long long)s.tiles * s.L;
+    const int per = (B + kThreads - 1) / kThreads, b0 = tid * per;
+    const Seq s0 = seq(b0);
+    // the work as a float: it only sets C, the same in every block
+    float work = (float)s0.tiles * (float)s0.L;
+    for (int i = 1; i < per; i++) {
+        const Seq s = seq(b0 + i);
+        work += (float)s.tiles * (float)s.L;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
-    if (lane == 0) s_sum[2][wave] = work;
+    if (lane == 0) s_work[wave] = work;
     __syncthreads();
-    work = 0;
+    work = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) work += s_sum[2][w];
-    long long C = (work * a.Hk + a.target - 1) / a.target;
-    C = (max(C, (long long)a.c_min) + kTile - 1) / kTile * kTile;
-    auto splits = [&](const Seq& s) {
-        return max(1, (int)((s.L + C / 2) / C));
-    };
-    long long units = 0, parts = 0;
-    for (int b = b0; b < b1; b++) {
-        const Seq s = seq(b);
-        const int ns = splits(s);
-        units += (long long)s.tiles * a.Hk * ns;
-        if (ns > 1) parts += (long long)s.tiles * a.Hk * ns;
+    for (int w = 0; w < kWaves; w++) work += s_work[w];
+    const uint32_t cf = (uint32_t)fminf(work * (float)a.Hk / (float)a.target, 1.0e9f);
+    const uint32_t C = (max(cf + 1, (uint32_t)a.c_min) + kTile - 1) / kTile * kTile;
+    auto splits = [&](const Seq& s) { return max(1u, ((uint32_t)s.L + C / 2) / C); };
+    const uint32_t ns0 = splits(s0), here0 = s0.tiles * a.Hk * ns0;
+    uint32_t units = here0, parts = ns0 > 1 ? here0 : 0;
+    for (int i = 1; i < per; i++) {
+        const Seq s = seq(b0 + i);
+        const uint32_t ns = splits(s), h = s.tiles * a.Hk * ns;
+        units += h;
+        parts += ns > 1 ? h : 0;
     }
-    long long iu = units, ip = parts;
+    uint32_t iu = units, ip = parts;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const long long x = __shfl_up(iu, o), y = __shfl_up(ip, o);
+        const uint32_t x = __shfl_up(iu, o), y = __shfl_up(ip, o);
         if (lane >= o) {
             iu += x;
             ip += y;
@@ -288,39 +325,37 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
         s_sum[1][wave] = ip;
     }
     __syncthreads();
-    long long pu = iu - units, pp = ip - parts;
+    uint32_t pu = iu - units, pp = ip - parts;
 #pragma unroll
     for (int w = 0; w < kWaves; w++)
         if (w < wave) {
             pu += s_sum[0][w];
             pp += s_sum[1][w];
         }
-    const long long me = blockIdx.x;
-    if (me >= pu && me < pu + units) {
-        for (int b = b0; b < b1; b++) {
-            const Seq s = seq(b);
-            const int ns = splits(s);
-            const long long here = (long long)s.tiles * a.Hk * ns;
-            if (me < pu + here) {
+    const uint32_t me = blockIdx.x;
+    if (me >= pu && me - pu < units) {
+        for (int i = 0; i < per; i++) {
+            const Seq s = i ? seq(b0 + i) : s0;
+            const uint32_t ns = i ? splits(s) : ns0, here = s.tiles * a.Hk * ns;
+            if (me - pu < here) {
                 // KV heads fastest: with 8 of them a head's pieces share an XCD's L2
-                const int x = (int)(me - pu), y = x / a.Hk;
+                const uint32_t x = me - pu, y = x / a.Hk;
                 Unit f;
-                f.b = b;
-                f.hk = x % a.Hk;
-                f.tile = y % s.tiles;
-                f.split = y / s.tiles;
-                f.nsplit = ns;
+                f.b = b0 + i;
+                f.hk = (int)(x - y * a.Hk);
+                f.split = (int)(y / s.tiles);
+                f.tile = (int)(y - (uint32_t)f.split * s.tiles);
+                f.nsplit = (int)ns;
                 f.L = s.L;
                 f.n = s.n;
                 f.r0 = s.r0;
-                const long long first = pp;
+                const uint32_t first = min(pp, (uint32_t)a.max_parts);
                 f.part = -1;
                 if (ns > 1) {
-                    const long long at = first + ((long long)f.hk * s.tiles + f.tile) * ns + f.split;
-                    f.part = at < a.max_parts ? (int)at : -2;
+                    const unsigned long long at = first + ((unsigned long long)f.hk * s.tiles + f.tile) * ns + f.split;
+                    f.part = at < (unsigned)a.max_parts ? (int)at : -2;
                 }
-                if (x == 0)
-                    a.info[b] = make_int4(ns, (int)min(first, (long long)a.max_parts), s.tiles, TROWS);
+                if (x == 0) a.info[f.b] = make_int4((int)ns, (int)first, s.tiles, TROWS);
                 s_unit = f;
                 break;
             }
@@ -347,8 +382,8 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
 // wave; KS: the block's waves share the rows and take the tiles of 32 keys in
 // turn (few rows, the sums joined in LDS), else each wave has rows of its own
 // over all of the unit's keys.
-template <int NC, int NG, int RT, bool KS>
-__global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
+template <int NC, int NG, int RT, bool KS, int WPS>
+__global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
     constexpr int D = 32 * NC, half = D / 2, TROWS = 16 * RT * (KS ? 1 : kWaves);
     constexpr int GD = D / NG, TPG = GD / 16, NT = D / 16;   // dims, O tiles a group; O tiles
     constexpr int QW = KS ? 1 : kWaves;
@@ -360,6 +395,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4, G = a.H / a.Hk, R = u.n * G, L = u.L;
     const int row0 = u.tile * TROWS + (KS ? 0 : wave * 16 * RT);
+    const Nib nib = nib_consts();
     const int hk = u.hk, b = u.b, lp = a.lp, pmask = (1 << lp) - 1;
 
     // chain: keys up to base + i; tree: keys below base and those of the bits
@@ -419,17 +455,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
         int e = (int)(__float_as_uint(top) >> 23) - 127;
         e = min(max(e, -100), 127);
         qinv[rt] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-        const int up = 14 - e;
+        const float up = __uint_as_float((uint32_t)(min(14 - e, 127) + 127) << 23);
         if (KS && wave != rt) continue;          // shared rows: one writer
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            f16x8 hi, lo;
+            float x[8];
 #pragma unroll
-            for (int p = 0; p < 8; p++) {
-                const float x = ldexpf(v[c][slot_of(p)], up);
-                hi[p] = (_Float16)x;
-                lo[p] = (_Float16)(x - (float)hi[p]);
-            }
+            for (int p = 0; p < 8; p++) x[p] = v[c][slot_of(p)];
+            f16x8 hi, lo;
+            split8(x, up, hi, lo);
             s_q[KS ? 0 : wave][rt][c][0][lane] = hi;
             s_q[KS ? 0 : wave][rt][c][1][lane] = lo;
         }
@@ -515,7 +549,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
                 for (int rt = 0; rt < RT; rt++) acc[rt] = (f32x4)(0.0f);
 #pragma unroll
                 for (int c = y * NC / NG; c < (y + 1) * NC / NG; c++) {
-                    const f16x8 kc = codes8(td.k[h][c] ^ 0x88888888u);
+                    const f16x8 kc = codes8(td.k[h][c] ^ 0x88888888u, nib);
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++) {
                         acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[KS ? 0 : wave][rt][c][0][ql], acc[rt], 0, 0, 0);
@@ -587,18 +621,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
                 const int en = max(max(et, ew[rt][y] - whole[rt]), -100);
                 const float f = __builtin_amdgcn_exp2f((float)(ew[rt][y] - en) - drop[rt]);
                 ew[rt][y] = en;
-                const float up = __uint_as_float((uint32_t)(14 - en + 127) << 23);
-#pragma unroll
-                for (int p = 0; p < 8; p++) {
-                    const float x = w[p] * up;
-                    hi[rt][p] = (_Float16)x;
-                    lo[rt][p] = (_Float16)(x - (float)hi[rt][p]);
-                }
+                split8(w, __uint_as_float((uint32_t)(14 - en + 127) << 23), hi[rt], lo[rt]);
                 if (__any(f != 1.0f)) {
 #pragma unroll
                     for (int t = 0; t < TPG; t++) o[rt][y * TPG + t] *= f;
                 }
             }
+            uint32_t vw[2][NC];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) vw[h][c] = td.v[h][y][c] ^ 0x88888888u;
 #pragma unroll
             for (int t = 0; t < TPG; t++) {
                 const uint32_t at = (uint32_t)(beta[y] + t / 2) * 0x10001u;
@@ -608,11 +641,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
                 f16x8 va;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const uint32_t (&v)[NC] = td.v[h][y];
-                    const uint32_t w01 = __builtin_amdgcn_perm(v[NC > 2 ? 1 : 0], v[0], s01) ^ 0x00880088u;
-                    const uint32_t w23 = __builtin_amdgcn_perm(v[NC > 2 ? b23 + 1 : b23], v[b23], s23) ^ 0x00880088u;
-                    const f16x2 x = t & 1 ? high_nibbles(w01) : low_nibbles(w01);
-                    const f16x2 z = t & 1 ? high_nibbles(w23) : low_nibbles(w23);
+                    const uint32_t (&v)[NC] = vw[h];
+                    const uint32_t w01 = __builtin_amdgcn_perm(v[NC > 2 ? 1 : 0], v[0], s01);
+                    const uint32_t w23 = __builtin_amdgcn_perm(v[NC > 2 ? b23 + 1 : b23], v[b23], s23);
+                    const f16x2 x = t & 1 ? high_nibbles(w01, nib) : low_nibbles(w01, nib);
+                    const f16x2 z = t & 1 ? high_nibbles(w23, nib) : low_nibbles(w23, nib);
                     va[4 * h] = x[0]; va[4 * h + 1] = x[1]; va[4 * h + 2] = z[0]; va[4 * h + 3] = z[1];
                 }
 #pragma unroll
@@ -746,7 +779,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_paged(PagedArgs a) {
 // Joins the pieces of split rows: block = (row, head), its waves take pieces
 // in turn; m relative to the largest of the pieces, as in the block itself.
 __global__ __launch_bounds__(kThreads) void k_paged_join(PagedArgs a) {
-    __shared__ float s_o[kWaves][128], s_l[kWaves], s_m[kWaves];
+    __shared__ float s_o[kWaves][128], s_l[kWaves];
     const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = a.row_seq[t];
     if (b < 0 || b >= a.seqs) return;
@@ -761,26 +794,45 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(PagedArgs a) {
     if (tile >= tiles || at + ns > a.max_parts) return;
     const size_t p0 = (size_t)at * trows + (r - tile * trows);
     const int D = a.D;
+    // every wave finds the maximum; the pieces' weights go to LDS 64 at a time,
+    // then a wave adds its share of them with all its loads in flight
     float M = -INFINITY;
     for (int s = lane; s < ns; s += 64) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * trows)]);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    const int d = 2 * lane;
-    for (int s = wave; s < ns; s += kWaves) {
-        const size_t p = p0 + (size_t)s * trows;
-        const float mw = a.part_ml[2 * p], w = mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M);
-        l += w * a.part_ml[2 * p + 1];
-        if (d < D) {
-            const f32x2 v = *(const f32x2*)(a.part_o + p * D + d);
-            o0 += w * v.x;
-            o1 += w * v.y;
+    const int d = min(2 * lane, D - 2);
+    for (int s0 = 0; s0 < ns; s0 += 64) {
+        const int s = s0 + lane;
+        float w = 0.0f;
+        if (s < ns) {
+            const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (p0 + (size_t)s * trows));
+            w = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            if (wave == 0) l += w * ml.y;
+        }
+        const int end = min(64, ns - s0);
+#pragma unroll 1
+        for (int k0 = 4 * wave; k0 < end; k0 += 16) {
+            f32x2 v[4];
+            float f[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int k = min(k0 + x, end - 1);
+                f[x] = k0 + x < end ? __shfl(w, k) : 0.0f;
+                v[x] = *(const f32x2*)(a.part_o + (p0 + (size_t)(s0 + k) * trows) * D + d);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                if (k0 + x < end) {
+                    o0 += f[x] * v[x].x;
+                    o1 += f[x] * v[x].y;
+                }
         }
     }
-    if (d < D) {
-        s_o[wave][d] = o0;
-        s_o[wave][d + 1] = o1;
-    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+    s_o[wave][d] = o0;
+    s_o[wave][d + 1] = o1;
     if (lane == 0) s_l[wave] = l;
     __syncthreads();
     l = 0.0f;
@@ -837,10 +889,10 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
         l.target = target;
         // round(len / C) pieces: at most target units by length and one a tile
         const long long whole = tiles * c->n_heads, pieces = (keys + c_min / 2) / c_min;
-        l.grid = whole + target;
+        l.grid = whole + target + 8;             // 8: C is rounded in 32 bits
         if (l.grid > whole * (pieces < 1 ? 1 : pieces)) l.grid = whole * (pieces < 1 ? 1 : pieces);
         // a split tile has at least 1.5 C keys, so at most 4/3 target pieces in all
-        l.max_parts = pieces > 1 ? target * 4 / 3 + 1 : 0;
+        l.max_parts = pieces > 1 ? target * 4 / 3 + 8 : 0;
         if (l.max_parts > l.grid) l.max_parts = (int)l.grid;
         l.part_o = (size_t)l.max_parts * trows * D * 4;
         l.part_ml = (size_t)l.max_parts * trows * 2 * 4;
@@ -848,18 +900,23 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     };
     p.info = (size_t)s->seqs * sizeof(int4);
     p.total = p.info;
-    add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 1024);
-    if (R > kSplitRows)
-        add(2, false, kSplitRows + 1, 0x7fffffff, ((long long)s->rows * G) / 128 + seqs, 256, 256);
+    // one sequence: one launch, whichever its bound on the rows asks for
+    const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
+    if (!tiles || both)
+        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 896);
+    if (tiles)
+        add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 128 + seqs,
+            256, 512);
     return p;
 }
 
 template <int NC, int NG>
 void launch_shape(const Launch& l, const PagedArgs& a) {
+    constexpr int WPS1 = NG == 1 ? 3 : 2;
     const dim3 grid((unsigned)l.grid), block(kThreads);
-    if (l.rt == 1) hipLaunchKernelGGL((k_attn_paged<NC, NG, 1, true>), grid, block, 0, stream(), a);
-    else if (l.rt == 2) hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, true>), grid, block, 0, stream(), a);
-    else hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, false>), grid, block, 0, stream(), a);
+    if (l.rt == 1) hipLaunchKernelGGL((k_attn_paged<NC, NG, 1, true, WPS1>), grid, block, 0, stream(), a);
+    else if (l.rt == 2) hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, true, 2>), grid, block, 0, stream(), a);
+    else hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, false, 2>), grid, block, 0, stream(), a);
 }
 
 void launch(const Launch& l, const PagedArgs& a) {
