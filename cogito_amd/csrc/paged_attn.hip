@@ -256,21 +256,41 @@ struct Unit {
     int b, hk, tile, split, nsplit, part, L, n, r0;
 };
 
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {      // inclusive scan over the wave
+#define CGX_ROW(CTRL, RMASK) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, RMASK, 0xF, true)
+    CGX_ROW(0x111, 0xF);
+    CGX_ROW(0x112, 0xF);
+    CGX_ROW(0x114, 0xF);
+    CGX_ROW(0x118, 0xF);
+    CGX_ROW(0x142, 0xA);
+    CGX_ROW(0x143, 0xC);
+#undef CGX_ROW
+    return v;
+}
+__device__ __forceinline__ float dpp_total(float v) {          // the wave's sum, in every lane
+#define CGX_ROW(CTRL, RMASK) \
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, RMASK, 0xF, true))
+    CGX_ROW(0x111, 0xF);
+    CGX_ROW(0x112, 0xF);
+    CGX_ROW(0x114, 0xF);
+    CGX_ROW(0x118, 0xF);
+    CGX_ROW(0x142, 0xA);
+    CGX_ROW(0x143, 0xC);
+#undef CGX_ROW
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
 // The block's unit of work: sequences of r_lo .. r_hi rows in order, each with
 // Hk * tiles * nsplit units.  The chunk length C follows from the keys of all
 // of them, so that there are about `target` units whatever the lengths; a
-// sequence is cut into round(len / C) even pieces.  Every block finds this out
-// for itself from the lengths: a few hundred words, against a launch more and
-// a wait for it.
+// sequence is cut into round(len / C) even pieces.  Every wave finds this out
+// for itself from the lengths, a lane taking B / 64 sequences: no LDS, no
+// barrier, against a launch more and a wait for it.
 //
 // The counts are 32 bits: consistent lengths stay below the grid, and others
 // may wrap, where a unit is only ever one that some sequence has.
-template <int TROWS>
-__device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
-    __shared__ float s_work[kWaves];
-    __shared__ uint32_t s_sum[2][kWaves];
-    __shared__ Unit s_unit;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = a.seqs, G = a.H / a.Hk;
+__device__ __forceinline__ bool find_unit(const PagedArgs& a, int trows, Unit& u) {
+    const int lane = threadIdx.x & 63, B = a.seqs, G = a.H / a.Hk;
     const long long most = (long long)a.table_ld << a.lp;
     struct Seq { int r0, n, L, tiles; };
     auto seq = [&](int b) {
@@ -281,25 +301,18 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
         s.n = max(0, min(r1, a.rows) - s.r0);
         s.L = (int)min((long long)max(kv, 0), most);
         const long long R = (long long)s.n * G;
-        s.tiles = R >= a.r_lo && R <= a.r_hi ? (int)((R + TROWS - 1) / TROWS) : 0;
+        s.tiles = R >= a.r_lo && R <= a.r_hi ? (int)((R + trows - 1) / trows) : 0;
         return s;
     };
-    if (tid == 0) s_unit.b = -1;
-    const int per = (B + kThreads - 1) / kThreads, b0 = tid * per;
+    const int per = (B + 63) >> 6, b0 = lane * per;
     const Seq s0 = seq(b0);
-    // the work as a float: it only sets C, the same in every block
+    // the work as a float: it only sets C, the same in every wave
     float work = (float)s0.tiles * (float)s0.L;
     for (int i = 1; i < per; i++) {
         const Seq s = seq(b0 + i);
         work += (float)s.tiles * (float)s.L;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
-    if (lane == 0) s_work[wave] = work;
-    __syncthreads();
-    work = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) work += s_work[w];
+    work = dpp_total(work);
     const uint32_t cf = (uint32_t)fminf(work * (float)a.Hk / (float)a.target, 1.0e9f);
     const uint32_t C = (max(cf + 1, (uint32_t)a.c_min) + kTile - 1) / kTile * kTile;
     auto splits = [&](const Seq& s) { return max(1u, ((uint32_t)s.L + C / 2) / C); };
@@ -311,90 +324,64 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, Unit& u) {
         units += h;
         parts += ns > 1 ? h : 0;
     }
-    uint32_t iu = units, ip = parts;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(iu, o), y = __shfl_up(ip, o);
-        if (lane >= o) {
-            iu += x;
-            ip += y;
-        }
-    }
-    if (lane == 63) {
-        s_sum[0][wave] = iu;
-        s_sum[1][wave] = ip;
-    }
-    __syncthreads();
-    uint32_t pu = iu - units, pp = ip - parts;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++)
-        if (w < wave) {
-            pu += s_sum[0][w];
-            pp += s_sum[1][w];
-        }
+    uint32_t pu = dpp_add(units) - units, pp = dpp_add(parts) - parts;
     const uint32_t me = blockIdx.x;
-    if (me >= pu && me - pu < units) {
-        for (int i = 0; i < per; i++) {
-            const Seq s = i ? seq(b0 + i) : s0;
-            const uint32_t ns = i ? splits(s) : ns0, here = s.tiles * a.Hk * ns;
-            if (me - pu < here) {
-                // KV heads fastest: with 8 of them a head's pieces share an XCD's L2
-                const uint32_t x = me - pu, y = x / a.Hk;
-                Unit f;
-                f.b = b0 + i;
-                f.hk = (int)(x - y * a.Hk);
-                f.split = (int)(y / s.tiles);
-                f.tile = (int)(y - (uint32_t)f.split * s.tiles);
-                f.nsplit = (int)ns;
-                f.L = s.L;
-                f.n = s.n;
-                f.r0 = s.r0;
-                const uint32_t first = min(pp, (uint32_t)a.max_parts);
-                f.part = -1;
-                if (ns > 1) {
-                    const unsigned long long at = first + ((unsigned long long)f.hk * s.tiles + f.tile) * ns + f.split;
-                    f.part = at < (unsigned)a.max_parts ? (int)at : -2;
-                }
-                if (x == 0) a.info[f.b] = make_int4((int)ns, (int)first, s.tiles, TROWS);
-                s_unit = f;
-                break;
-            }
+    const unsigned long long mine = __ballot(me >= pu && me - pu < units);
+    if (!mine) return false;
+    const int owner = __builtin_ctzll(mine);
+    // the owner's first sequence of the unit, then its fields to every lane
+    Seq s = s0;
+    int b = b0;
+    uint32_t ns = ns0, here = here0;
+    if (lane == owner)
+        while (me - pu >= here) {
             pu += here;
             if (ns > 1) pp += here;
+            s = seq(++b);
+            ns = splits(s);
+            here = s.tiles * a.Hk * ns;
         }
+    auto give = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+    u.b = give(b);
+    u.L = give(s.L);
+    u.n = give(s.n);
+    u.r0 = give(s.r0);
+    u.nsplit = give((int)ns);
+    const uint32_t tiles = (uint32_t)give(s.tiles), x = me - (uint32_t)give((int)pu), y = x / a.Hk;
+    const uint32_t first = min((uint32_t)give((int)pp), (uint32_t)a.max_parts);
+    // KV heads fastest: with 8 of them a head's pieces share an XCD's L2
+    u.hk = (int)(x - y * a.Hk);
+    u.split = (int)(y / tiles);
+    u.tile = (int)(y - (uint32_t)u.split * tiles);
+    u.part = -1;
+    if (u.nsplit > 1) {
+        const unsigned long long at = first + ((unsigned long long)u.hk * tiles + u.tile) * u.nsplit + u.split;
+        u.part = at < (unsigned)a.max_parts ? (int)at : -2;
     }
-    __syncthreads();
-    u = s_unit;
-    // the same in every lane: scalars
-    u.b = __builtin_amdgcn_readfirstlane(u.b);
-    u.hk = __builtin_amdgcn_readfirstlane(u.hk);
-    u.tile = __builtin_amdgcn_readfirstlane(u.tile);
-    u.split = __builtin_amdgcn_readfirstlane(u.split);
-    u.nsplit = __builtin_amdgcn_readfirstlane(u.nsplit);
-    u.part = __builtin_amdgcn_readfirstlane(u.part);
-    u.L = __builtin_amdgcn_readfirstlane(u.L);
-    u.n = __builtin_amdgcn_readfirstlane(u.n);
-    u.r0 = __builtin_amdgcn_readfirstlane(u.r0);
-    return u.b >= 0;
+    if (x == 0 && threadIdx.x == 0) a.info[u.b] = make_int4(u.nsplit, (int)first, (int)tiles, trows);
+    return true;
 }
 
-// One unit.  NC = D / 32, NG scales a head row, RT tiles of 16 query rows a
-// wave; KS: the block's waves share the rows and take the tiles of 32 keys in
-// turn (few rows, the sums joined in LDS), else each wave has rows of its own
-// over all of the unit's keys.
-template <int NC, int NG, int RT, bool KS, int WPS>
-__global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
-    constexpr int D = 32 * NC, half = D / 2, TROWS = 16 * RT * (KS ? 1 : kWaves);
+// One unit.  NC = D / 32, NG scales a head row; the block's waves are RG groups
+// of 16 RT query rows times KG that take the tiles of 32 keys in turn, their
+// sums joined in LDS.
+template <int NC, int NG, int RT, int RG, int KG, int WPS>
+__global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
+    constexpr int D = 32 * NC, half = D / 2, TROWS = 16 * RT * RG;
     constexpr int GD = D / NG, TPG = GD / 16, NT = D / 16;   // dims, O tiles a group; O tiles
-    constexpr int QW = KS ? 1 : kWaves;
-    __shared__ f16x8 s_q[QW][RT][NC][2][64];
-    __shared__ float s_o[KS ? kWaves / 2 : 1][KS ? 16 * RT : 1][KS ? D + 4 : 1];
-    __shared__ float s_ml[KS ? kWaves : 1][KS ? 16 * RT : 1][2];
+    constexpr int kQBytes = RG * RT * NC * 2 * 64 * (int)sizeof(f16x8);
+    constexpr int kOBytes = KG / 2 * TROWS * (D + 4) * (int)sizeof(float);
+    // the Q operands, and when the tiles are done, the waves' O
+    __shared__ __attribute__((aligned(16))) unsigned char s_raw[kQBytes > kOBytes ? kQBytes : kOBytes];
+    f16x8 (*s_q)[RT][NC][2][64] = (f16x8 (*)[RT][NC][2][64])s_raw;
+    float (*s_o)[TROWS][D + 4] = (float (*)[TROWS][D + 4])s_raw;
+    __shared__ float s_ml[KG][TROWS][2];
     Unit u;
-    if (!find_unit<TROWS>(a, u)) return;
+    if (!find_unit(a, TROWS, u)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = wave % KG, rg = wave / KG;
     const int n = lane & 15, g = lane >> 4, G = a.H / a.Hk, R = u.n * G, L = u.L;
-    const int row0 = u.tile * TROWS + (KS ? 0 : wave * 16 * RT);
+    const int row0 = u.tile * TROWS + rg * 16 * RT;
     const Nib nib = nib_consts();
     const int hk = u.hk, b = u.b, lp = a.lp, pmask = (1 << lp) - 1;
 
@@ -456,7 +443,7 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
         e = min(max(e, -100), 127);
         qinv[rt] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
         const float up = __uint_as_float((uint32_t)(min(14 - e, 127) + 127) << 23);
-        if (KS && wave != rt) continue;          // shared rows: one writer
+        if (kg != rt % KG) continue;             // the group's rows: one writer
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             float x[8];
@@ -464,8 +451,8 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
             for (int p = 0; p < 8; p++) x[p] = v[c][slot_of(p)];
             f16x8 hi, lo;
             split8(x, up, hi, lo);
-            s_q[KS ? 0 : wave][rt][c][0][lane] = hi;
-            s_q[KS ? 0 : wave][rt][c][1][lane] = lo;
+            s_q[rg][rt][c][0][lane] = hi;
+            s_q[rg][rt][c][1][lane] = lo;
         }
     }
     __syncthreads();
@@ -484,7 +471,10 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
         f32x4 ks[2][NG], vs[2][NG];
         int ok;                                  // bit h: half h's page is in the pool
     };
-    const int* tab = a.table + (size_t)b * a.table_ld;
+    // page numbers by scalar loads (nobody writes the table while this runs):
+    // as vector loads each would wait for the tile in flight
+    typedef const __attribute__((address_space(4))) int* scalar_ints;
+    const scalar_ints tab = (scalar_ints)(uintptr_t)(a.table + (size_t)b * a.table_ld);
     struct Pages { int p[2]; };
     auto pages = [&](int kt) {
         Pages x;
@@ -552,8 +542,8 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
                     const f16x8 kc = codes8(td.k[h][c] ^ 0x88888888u, nib);
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++) {
-                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[KS ? 0 : wave][rt][c][0][ql], acc[rt], 0, 0, 0);
-                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[KS ? 0 : wave][rt][c][1][ql], acc[rt], 0, 0, 0);
+                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[rg][rt][c][0][ql], acc[rt], 0, 0, 0);
+                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[rg][rt][c][1][ql], acc[rt], 0, 0, 0);
                     }
                 }
 #pragma unroll
@@ -657,33 +647,35 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
         }
     };
 
-    constexpr int step = KS ? kWaves * kTile : kTile;
-    int kt = k_begin + (KS ? wave * kTile : 0);
-    if constexpr (NG == 1) {
+    constexpr int step = KG * kTile;
+    int kt = k_begin + kg * kTile;
+    if constexpr (NC * NG <= 4) {
+        // two tiles in turn: one is loaded while the other is multiplied (past
+        // the end page 0's first rows, which nobody looks at)
         if (kt < end) {
-            Tile cur, nxt;
-            load(kt, pages(kt), cur);
+            Tile x, y;
+            load(kt, pages(kt), x);
             Pages ahead = pages(kt + step);
             for (;;) {
-                const int next = kt + step;
-                if (next >= end) break;
-                load(next, ahead, nxt);
-                ahead = pages(next + step);
-                process(cur, kt);
-                cur = nxt;
-                kt = next;
+                load(kt + step, ahead, y);
+                ahead = pages(kt + 2 * step);
+                process(x, kt);
+                if ((kt += step) >= end) break;
+                load(kt + step, ahead, x);
+                ahead = pages(kt + 2 * step);
+                process(y, kt);
+                if ((kt += step) >= end) break;
             }
-            process(cur, kt);
         }
     } else {
-        // the scales and words of several groups leave no registers for a
+        // the words and scales of several groups leave no registers for a
         // second tile
         Pages ahead = pages(kt);
         for (; kt < end; kt += step) {
-            Tile cur;
-            load(kt, ahead, cur);
+            Tile x;
+            load(kt, ahead, x);
             ahead = pages(kt + step);
-            process(cur, kt);
+            process(x, kt);
         }
     }
 
@@ -710,53 +702,54 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
                     *(f32x2*)(to + dim(y, x) + t) = (f32x2){v[y * TPG + t][x] * f, v[y * TPG + t + 1][x] * f};
     };
 
-    if constexpr (KS) {
-        // the waves' maxima and sums, then O of waves 2, 3 onto 0, 1, and 1 onto 0
-        if (g == 0) {
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                s_ml[wave][16 * rt + n][0] = m[rt];
-                s_ml[wave][16 * rt + n][1] = l[rt];
-            }
-        }
-        __syncthreads();
+    // the key groups' maxima and sums, then O of the upper half of them onto
+    // the lower until one is left
+    const int lr = rg * 16 * RT + n;             // the row's place in the tile, plus 16 rt
+    if (g == 0) {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            float M = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) M = fmaxf(M, s_ml[w][16 * rt + n][0]);
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                const float mw = s_ml[w][16 * rt + n][0];
-                sum += s_ml[w][16 * rt + n][1] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
-            }
-            const float f = m[rt] == M ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - M);
-            m[rt] = M;
-            l[rt] = sum;
-#pragma unroll
-            for (int t = 0; t < NT; t++) o[rt][t] *= f;
+            s_ml[kg][lr + 16 * rt][0] = m[rt];
+            s_ml[kg][lr + 16 * rt][1] = l[rt];
         }
-#pragma unroll
-        for (int from = kWaves / 2; from > 0; from >>= 1) {
-            if (wave >= from && wave < 2 * from) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) put(&s_o[wave - from][16 * rt + n][0], o[rt], 1.0f);
-            }
-            __syncthreads();
-            if (wave < from) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int y = 0; y < NG; y++)
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-#pragma unroll
-                            for (int t = 0; t < TPG; t++) o[rt][y * TPG + t][x] += s_o[wave][16 * rt + n][dim(y, x) + t];
-            }
-            __syncthreads();
-        }
-        if (wave != 0) return;
     }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KG; w++) M = fmaxf(M, s_ml[w][lr + 16 * rt][0]);
+#pragma unroll
+        for (int w = 0; w < KG; w++) {
+            const float mw = s_ml[w][lr + 16 * rt][0];
+            sum += s_ml[w][lr + 16 * rt][1] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+        }
+        const float f = m[rt] == M ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - M);
+        m[rt] = M;
+        l[rt] = sum;
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[rt][t] *= f;
+    }
+#pragma unroll
+    for (int from = KG / 2; from > 0; from >>= 1) {
+        if (kg >= from && kg < 2 * from) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) put(&s_o[kg - from][lr + 16 * rt][0], o[rt], 1.0f);
+        }
+        __syncthreads();
+        if (kg < from) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int y = 0; y < NG; y++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int t = 0; t < TPG; t++)
+                            o[rt][y * TPG + t][x] += s_o[kg][lr + 16 * rt][dim(y, x) + t];
+        }
+        if (from > 1) __syncthreads();
+    }
+    if (kg) return;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         if (!rok[rt] || u.part == -2) continue;
@@ -766,7 +759,7 @@ __global__ __launch_bounds__(kThreads, WPS) void k_attn_paged(PagedArgs a) {
             if (a.lse && g == 0)
                 a.lse[qrow[rt]] = l[rt] != 0.0f ? 0.69314718055994530942f * (m[rt] + log2f(l[rt])) : -INFINITY;
         } else {
-            const size_t pr = (size_t)u.part * TROWS + (row0 - u.tile * TROWS) + 16 * rt + n;
+            const size_t pr = (size_t)u.part * TROWS + lr + 16 * rt;
             put(a.part_o + pr * D, o[rt], 1.0f);
             if (g == 0) {
                 a.part_ml[2 * pr] = m[rt];
@@ -881,7 +874,7 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     const long long keys = (long long)s->table_ld * c->page_size;
     auto add = [&](int rt, bool ks, int lo, long long hi, long long tiles, int c_min, int target) {
         Launch& l = p.l[p.n++];
-        const int trows = 16 * rt * (ks ? 1 : kWaves);
+        const int trows = 16 * rt * (ks ? 1 : 2);
         l.rt = ks ? rt : -rt;
         l.r_lo = lo;
         l.r_hi = (int)(hi > 0x7fffffff ? 0x7fffffff : hi);
@@ -903,20 +896,21 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     // one sequence: one launch, whichever its bound on the rows asks for
     const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
     if (!tiles || both)
-        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 896);
+        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 768);
     if (tiles)
-        add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 128 + seqs,
-            256, 512);
+        add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 64 + seqs,
+            256, 256);
     return p;
 }
 
 template <int NC, int NG>
 void launch_shape(const Launch& l, const PagedArgs& a) {
-    constexpr int WPS1 = NG == 1 ? 3 : 2;
-    const dim3 grid((unsigned)l.grid), block(kThreads);
-    if (l.rt == 1) hipLaunchKernelGGL((k_attn_paged<NC, NG, 1, true, WPS1>), grid, block, 0, stream(), a);
-    else if (l.rt == 2) hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, true, 2>), grid, block, 0, stream(), a);
-    else hipLaunchKernelGGL((k_attn_paged<NC, NG, 2, false, 2>), grid, block, 0, stream(), a);
+    // the words and scales of NC NG > 4 take the registers of a second row tile
+    constexpr int RT = NC * NG > 4 ? 1 : 2, S = 2 / RT;
+    const dim3 grid((unsigned)l.grid);
+    if (l.rt == 1) hipLaunchKernelGGL((k_attn_paged<NC, NG, 1, 1, 4, (NC * NG > 4 ? 2 : 3)>), grid, dim3(256), 0, stream(), a);
+    else if (l.rt == 2) hipLaunchKernelGGL((k_attn_paged<NC, NG, RT, S, 4 / S, 2>), grid, dim3(256), 0, stream(), a);
+    else hipLaunchKernelGGL((k_attn_paged<NC, NG, RT, 2 * S, 4 / S, 2>), grid, dim3(512), 0, stream(), a);
 }
 
 void launch(const Launch& l, const PagedArgs& a) {
