@@ -14,6 +14,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "cgx_internal.h"
 
@@ -56,11 +57,14 @@ struct PagedArgs {
     float* lse;
     // k_attn_paged: sequences of r_lo .. r_hi query rows times heads a KV
     // head, key chunks of at least c_min, about `target` units; partial
-    // results of split tiles and what k_paged_join needs of each sequence
+    // results of split tiles (this launch's from row part_row on, at most
+    // max_parts tiles of rows) and where k_paged_join finds those of a row
     int r_lo, r_hi, c_min, target, max_parts;
-    float* part_o;               // [parts][tile rows][D]
-    float* part_ml;              // [parts][tile rows][2]
-    int4* info;                  // [seqs] splits, first part, tiles, tile rows
+    long long part_row, part_rows;
+    float* part_o;               // [part_rows][D]
+    float* part_ml;              // [part_rows][2]
+    int4* info;                  // [rows] pieces, part_row of the first tile (two words),
+                                 // place among the sequence's rows; then [rows] tiles, tile rows
 };
 
 __device__ __forceinline__ float code(unsigned n) { return (float)((int)(n << 28) >> 28); }
@@ -253,7 +257,7 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
 }
 
 struct Unit {
-    int b, hk, tile, split, nsplit, part, L, n, r0;
+    int b, hk, tile, split, nsplit, part, first, tiles, L, n, r0;
 };
 
 __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {      // inclusive scan over the wave
@@ -349,6 +353,8 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, int trows, Unit& u
     u.nsplit = give((int)ns);
     const uint32_t tiles = (uint32_t)give(s.tiles), x = me - (uint32_t)give((int)pu), y = x / a.Hk;
     const uint32_t first = min((uint32_t)give((int)pp), (uint32_t)a.max_parts);
+    u.first = (int)first;
+    u.tiles = (int)tiles;
     // KV heads fastest: with 8 of them a head's pieces share an XCD's L2
     u.hk = (int)(x - y * a.Hk);
     u.split = (int)(y / tiles);
@@ -358,8 +364,14 @@ __device__ __forceinline__ bool find_unit(const PagedArgs& a, int trows, Unit& u
         const unsigned long long at = first + ((unsigned long long)u.hk * tiles + u.tile) * u.nsplit + u.split;
         u.part = at < (unsigned)a.max_parts ? (int)at : -2;
     }
-    if (x == 0 && threadIdx.x == 0) a.info[u.b] = make_int4(u.nsplit, (int)first, (int)tiles, trows);
     return true;
+}
+
+// Barrier for LDS alone: loads from memory in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // One unit.  NC = D / 32, NG scales a head row; the block's waves are RG groups
@@ -413,49 +425,6 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     end = min(end, min(L, k_begin + piece));
     const int first_i = row0 < R ? row0 / G : 0;
     const int open_end = row0 < R ? min(L, a.anc ? base : base + first_i + 1) : 0;
-
-    // ---- Q^T operands: element p of chunk c is dim (NG == 1) g D/4 + 8 c +
-    //      slot, (NG > 1) 32 c + 8 g + slot, so that a product never spans
-    //      two scale groups
-    float qinv[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const float* q = a.Q + qrow[rt] * D;
-        float v[NC][8], top = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int x = 0; x < 8; x += 4) {
-                const float4 t = *(const float4*)(q + (NG == 1 ? g * (D / 4) + 8 * c : 32 * c + 8 * g) + x);
-                v[c][x] = t.x; v[c][x + 1] = t.y; v[c][x + 2] = t.z; v[c][x + 3] = t.w;
-            }
-        const float f = a.scale * 1.44269504088896340736f;
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int x = 0; x < 8; x++) {
-                v[c][x] = rok[rt] ? v[c][x] * f : 0.0f;
-                top = fmaxf(top, fabsf(v[c][x]));
-            }
-        top = max_rows(top);
-        // 2^e <= top < 2^(e + 1); far exponents are cut where fp16's range covers them
-        int e = (int)(__float_as_uint(top) >> 23) - 127;
-        e = min(max(e, -100), 127);
-        qinv[rt] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-        const float up = __uint_as_float((uint32_t)(min(14 - e, 127) + 127) << 23);
-        if (kg != rt % KG) continue;             // the group's rows: one writer
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            float x[8];
-#pragma unroll
-            for (int p = 0; p < 8; p++) x[p] = v[c][slot_of(p)];
-            f16x8 hi, lo;
-            split8(x, up, hi, lo);
-            s_q[rg][rt][c][0][lane] = hi;
-            s_q[rg][rt][c][1][lane] = lo;
-        }
-    }
-    __syncthreads();
 
     // ---- V^T operands: group y's O tile t has dims y GD + TPG n + t of lane
     //      n, that is bytes beta .. of block blk of the V page
@@ -513,6 +482,59 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         }
     };
 
+    // ---- Q^T operands: element p of chunk c is dim (NG == 1) g D/4 + 8 c +
+    //      slot, (NG > 1) 32 c + 8 g + slot, so that a product never spans
+    //      two scale groups.  Q's loads come first, then the first tile's, so
+    //      that the operands are made while that is on its way.
+    float qv[RT][NC][8];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float* q = a.Q + qrow[rt] * D;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int x = 0; x < 8; x += 4) {
+                const float4 t = *(const float4*)(q + (NG == 1 ? g * (D / 4) + 8 * c : 32 * c + 8 * g) + x);
+                qv[rt][c][x] = t.x; qv[rt][c][x + 1] = t.y; qv[rt][c][x + 2] = t.z; qv[rt][c][x + 3] = t.w;
+            }
+    }
+    constexpr int step = KG * kTile;
+    int kt = k_begin + kg * kTile;
+    Tile x;
+    load(kt, pages(kt), x);
+    Pages ahead = pages(kt + step);
+    float qinv[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float f = a.scale * 1.44269504088896340736f;
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                qv[rt][c][i] = rok[rt] ? qv[rt][c][i] * f : 0.0f;
+                top = fmaxf(top, fabsf(qv[rt][c][i]));
+            }
+        top = max_rows(top);
+        // 2^e <= top < 2^(e + 1); far exponents are cut where fp16's range covers them
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = min(max(e, -100), 127);
+        qinv[rt] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+        const float up = __uint_as_float((uint32_t)(min(14 - e, 127) + 127) << 23);
+        if (kg != rt % KG) continue;             // the group's rows: one writer
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            float v[8];
+#pragma unroll
+            for (int p = 0; p < 8; p++) v[p] = qv[rt][c][slot_of(p)];
+            f16x8 hi, lo;
+            split8(v, up, hi, lo);
+            s_q[rg][rt][c][0][lane] = hi;
+            s_q[rg][rt][c][1][lane] = lo;
+        }
+    }
+    lds_barrier();
+
     float m[RT], l[RT];
     int ew[RT][NG];
     f32x4 o[RT][NT];
@@ -526,7 +548,9 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         for (int t = 0; t < NT; t++) o[rt][t] = (f32x4)(0.0f);
     }
 
-    auto process = [&](const Tile& td, int kt) {
+    // OPEN: every key of the tile is seen by every row
+    auto tile = [&](auto open, const Tile& td, int kt) {
+        constexpr bool OPEN = decltype(open)::value;
         int ql = lane;
         asm volatile("" : "+v"(ql));             // Q is read again each tile, not kept in registers
         f32x4 s[RT][2];
@@ -556,14 +580,13 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                     }
             }
         }
-        const bool open = td.ok == 3 && kt + kTile <= open_end && kt + kTile <= end;
         unsigned see[RT];
         float drop[RT], pr[RT][8];
         int whole[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             see[rt] = 0xffu;
-            if (!open) {
+            if constexpr (!OPEN) {
                 see[rt] = 0;
 #pragma unroll
                 for (int p = 0; p < 8; p++) {
@@ -603,7 +626,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                     const int e = (p & 3) * NG + y;
                     const float vs = td.vs[p >> 2][e / 4][e % 4];
                     // a hidden key's scale may be anything
-                    w[p] = open || ((see[rt] >> p) & 1) ? pr[rt][p] * vs : 0.0f;
+                    w[p] = OPEN || ((see[rt] >> p) & 1) ? pr[rt][p] * vs : 0.0f;
                     big = fmaxf(big, fabsf(w[p]));
                 }
                 big = max_rows(big);
@@ -647,36 +670,42 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         }
     };
 
-    constexpr int step = KG * kTile;
-    int kt = k_begin + kg * kTile;
+    // open tiles first, two in turn: one is loaded while the other is
+    // multiplied (past the end page 0's first rows, which nobody looks at);
+    // from the first tile on that is not open for all rows, one at a time
+    const int open_to = min(open_end, end) - kTile;
     if constexpr (NC * NG <= 4) {
-        // two tiles in turn: one is loaded while the other is multiplied (past
-        // the end page 0's first rows, which nobody looks at)
-        if (kt < end) {
-            Tile x, y;
-            load(kt, pages(kt), x);
-            Pages ahead = pages(kt + step);
-            for (;;) {
-                load(kt + step, ahead, y);
-                ahead = pages(kt + 2 * step);
-                process(x, kt);
-                if ((kt += step) >= end) break;
-                load(kt + step, ahead, x);
-                ahead = pages(kt + 2 * step);
-                process(y, kt);
-                if ((kt += step) >= end) break;
+        Tile y;
+        for (;;) {
+            if (kt > open_to || x.ok != 3) break;
+            load(kt + step, ahead, y);
+            ahead = pages(kt + 2 * step);
+            tile(std::true_type(), x, kt);
+            kt += step;
+            if (kt > open_to || y.ok != 3) {
+                x = y;
+                break;
             }
+            load(kt + step, ahead, x);
+            ahead = pages(kt + 2 * step);
+            tile(std::true_type(), y, kt);
+            kt += step;
         }
     } else {
         // the words and scales of several groups leave no registers for a
         // second tile
-        Pages ahead = pages(kt);
-        for (; kt < end; kt += step) {
-            Tile x;
+        while (kt <= open_to && x.ok == 3) {
+            tile(std::true_type(), x, kt);
+            kt += step;
             load(kt, ahead, x);
             ahead = pages(kt + step);
-            process(x, kt);
         }
+    }
+    while (kt < end) {
+        tile(std::false_type(), x, kt);
+        kt += step;
+        load(kt, ahead, x);
+        ahead = pages(kt + step);
     }
 
     // ---- row sums, and O back to one scale relative to m
@@ -712,7 +741,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
             s_ml[kg][lr + 16 * rt][1] = l[rt];
         }
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         float M = -INFINITY, sum = 0.0f;
@@ -735,7 +764,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) put(&s_o[kg - from][lr + 16 * rt][0], o[rt], 1.0f);
         }
-        __syncthreads();
+        lds_barrier();
         if (kg < from) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
@@ -747,19 +776,28 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                         for (int t = 0; t < TPG; t++)
                             o[rt][y * TPG + t][x] += s_o[kg][lr + 16 * rt][dim(y, x) + t];
         }
-        if (from > 1) __syncthreads();
+        if (from > 1) lds_barrier();
     }
     if (kg) return;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        if (!rok[rt] || u.part == -2) continue;
-        if (u.part < 0) {
+        if (!rok[rt]) continue;
+        if (a.part_rows && u.hk == 0 && u.split == 0 && g == 0) {
+            // one of the row's lanes says where its pieces are
+            const int r = row0 + 16 * rt + n, i = r / G;
+            if (r == i * G) {
+                const long long at = a.part_row + (long long)u.first * TROWS;
+                a.info[2 * (size_t)rq[rt]] = make_int4(u.nsplit, (int)at, (int)(at >> 32), i);
+                a.info[2 * (size_t)rq[rt] + 1] = make_int4(u.tiles, TROWS, 0, 0);
+            }
+        }
+        if (u.part == -1) {
             const float inv = l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f;
             put(a.O + qrow[rt] * D, o[rt], inv);
             if (a.lse && g == 0)
                 a.lse[qrow[rt]] = l[rt] != 0.0f ? 0.69314718055994530942f * (m[rt] + log2f(l[rt])) : -INFINITY;
-        } else {
-            const size_t pr = (size_t)u.part * TROWS + lr + 16 * rt;
+        } else if (u.part >= 0) {
+            const size_t pr = (size_t)a.part_row + (size_t)u.part * TROWS + lr + 16 * rt;
             put(a.part_o + pr * D, o[rt], 1.0f);
             if (g == 0) {
                 a.part_ml[2 * pr] = m[rt];
@@ -769,77 +807,75 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     }
 }
 
-// Joins the pieces of split rows: block = (row, head), its waves take pieces
-// in turn; m relative to the largest of the pieces, as in the block itself.
+// Joins the pieces of split rows: block = (row, every gridDim.y-th head), its
+// waves take pieces in turn; m relative to the largest of the pieces, as in
+// the block itself.  A row's place comes in one load, its pieces' sums and
+// values together in the next.
+constexpr int kJoin = 4;                         // pieces a wave loads at a time
 __global__ __launch_bounds__(kThreads) void k_paged_join(PagedArgs a) {
-    __shared__ float s_o[kWaves][128], s_l[kWaves];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = a.row_seq[t];
-    if (b < 0 || b >= a.seqs) return;
-    const int r0 = min(max(a.row_begin[b], 0), a.rows), i = t - r0;
-    const int n = max(0, min(a.row_begin[b + 1], a.rows) - r0), G = a.H / a.Hk;
-    if (i < 0 || i >= n || (long long)n * G < a.r_lo || (long long)n * G > a.r_hi) return;
-    const int4 f = a.info[b];
-    const int ns = f.x, tiles = f.z, trows = f.w;
-    if (ns < 2) return;
-    const int hk = h / G, r = i * G + (h - hk * G), tile = r / trows;
-    const long long at = f.y + ((long long)hk * tiles + tile) * ns;
-    if (tile >= tiles || at + ns > a.max_parts) return;
-    const size_t p0 = (size_t)at * trows + (r - tile * trows);
-    const int D = a.D;
-    // every wave finds the maximum; the pieces' weights go to LDS 64 at a time,
-    // then a wave adds its share of them with all its loads in flight
-    float M = -INFINITY;
-    for (int s = lane; s < ns; s += 64) M = fmaxf(M, a.part_ml[2 * (p0 + (size_t)s * trows)]);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    __shared__ float s_o[kWaves][128];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int4 f = a.info[2 * (size_t)t], f2 = a.info[2 * (size_t)t + 1];
+    const int b = a.row_seq[t], ns = f.x, tiles = f2.x, trows = f2.y, G = a.H / a.Hk, D = a.D;
+    // a row that no sequence has, or of a sequence left out, holds no word of this call
+    if (b < 0 || b >= a.seqs || ns < 2 || tiles < 1 || trows < 1 || f.w < 0) return;
+    const long long base = (long long)(uint32_t)f.y | (long long)f.z << 32;
     const int d = min(2 * lane, D - 2);
-    for (int s0 = 0; s0 < ns; s0 += 64) {
-        const int s = s0 + lane;
-        float w = 0.0f;
-        if (s < ns) {
-            const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (p0 + (size_t)s * trows));
-            w = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-            if (wave == 0) l += w * ml.y;
-        }
-        const int end = min(64, ns - s0);
-#pragma unroll 1
-        for (int k0 = 4 * wave; k0 < end; k0 += 16) {
-            f32x2 v[4];
-            float f[4];
+    for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
+        const int hk = h / G;
+        const uint32_t r = (uint32_t)f.w * G + (h - hk * G), tile = r / (uint32_t)trows;
+        const long long p0 = base + (long long)(((uint32_t)hk * tiles + tile) * (uint32_t)ns) * trows + (r - tile * trows);
+        if (base < 0 || tile >= (uint32_t)tiles || p0 + (long long)(ns - 1) * trows >= a.part_rows) return;
+        float M = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        for (int s0 = 0; s0 < ns; s0 += 64) {
+            const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (p0 + (long long)min(s0 + lane, ns - 1) * trows));
+            const int cnt = min(64, ns - s0);
+            f32x2 v[kJoin];
+            auto get = [&](int k0) {
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int k = min(k0 + x, end - 1);
-                f[x] = k0 + x < end ? __shfl(w, k) : 0.0f;
-                v[x] = *(const f32x2*)(a.part_o + (p0 + (size_t)(s0 + k) * trows) * D + d);
-            }
+                for (int x = 0; x < kJoin; x++)
+                    v[x] = *(const f32x2*)(a.part_o + (p0 + (long long)(s0 + min(k0 + x, cnt - 1)) * trows) * D + d);
+            };
+            get(kJoin * wave);
+            float top = ml.x;
 #pragma unroll
-            for (int x = 0; x < 4; x++)
-                if (k0 + x < end) {
-                    o0 += f[x] * v[x].x;
-                    o1 += f[x] * v[x].y;
+            for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+            const float mn = fmaxf(M, top), g = M == mn ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            const float w = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            l = l * g + (lane < cnt ? w * ml.y : 0.0f);
+            o0 *= g;
+            o1 *= g;
+            for (int k0 = kJoin * wave; k0 < cnt; k0 += kJoin * kWaves) {
+                f32x2 now[kJoin];
+#pragma unroll
+                for (int x = 0; x < kJoin; x++) now[x] = v[x];
+                if (k0 + kJoin * kWaves < cnt) get(k0 + kJoin * kWaves);
+#pragma unroll
+                for (int x = 0; x < kJoin; x++) {
+                    const float wx = __shfl(w, min(k0 + x, cnt - 1));
+                    if (k0 + x < cnt) {
+                        o0 += wx * now[x].x;
+                        o1 += wx * now[x].y;
+                    }
                 }
+            }
         }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+        s_o[wave][d] = o0;
+        s_o[wave][d + 1] = o1;
+        __syncthreads();
+        if ((int)threadIdx.x < D) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) v += s_o[w][threadIdx.x];
+            a.O[((size_t)t * a.H + h) * D + threadIdx.x] = l != 0.0f ? v / l : 0.0f;
+        }
+        if (a.lse && threadIdx.x == 0)
+            a.lse[(size_t)t * a.H + h] = l != 0.0f ? 0.69314718055994530942f * (M + log2f(l)) : -INFINITY;
+        __syncthreads();
     }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
-    s_o[wave][d] = o0;
-    s_o[wave][d + 1] = o1;
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) l += s_l[w];
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    for (int x = threadIdx.x; x < D; x += kThreads) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) v += s_o[w][x];
-        a.O[((size_t)t * a.H + h) * D + x] = v * inv;
-    }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[(size_t)t * a.H + h] = l != 0.0f ? 0.69314718055994530942f * (M + log2f(l)) : -INFINITY;
 }
 
 int log2i(int x) {
@@ -852,14 +888,14 @@ int log2i(int x) {
 // waves) and the tile launch (more rows, rows over the waves).
 struct Launch {
     int rt, r_lo, r_hi, c_min, target, max_parts;
-    long long grid;
-    size_t part_o, part_ml;      // bytes
+    long long grid, part_row;
 };
 struct Plan {
     bool fast;
     Launch l[2];
     int n;
-    size_t info, total;
+    long long part_rows;
+    size_t info, part_o, total;
 };
 
 constexpr int kSplitRows = 32;
@@ -887,19 +923,20 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
         // a split tile has at least 1.5 C keys, so at most 4/3 target pieces in all
         l.max_parts = pieces > 1 ? target * 4 / 3 + 8 : 0;
         if (l.max_parts > l.grid) l.max_parts = (int)l.grid;
-        l.part_o = (size_t)l.max_parts * trows * D * 4;
-        l.part_ml = (size_t)l.max_parts * trows * 2 * 4;
-        p.total += l.part_o + l.part_ml;
+        l.part_row = p.part_rows;
+        p.part_rows += (long long)l.max_parts * trows;
     };
-    p.info = (size_t)s->seqs * sizeof(int4);
-    p.total = p.info;
     // one sequence: one launch, whichever its bound on the rows asks for
     const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
     if (!tiles || both)
-        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, 768);
+        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, R > 16 ? 512 : 768);
     if (tiles)
         add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 64 + seqs,
             256, 256);
+    if (!p.part_rows) return p;
+    p.info = 2 * (size_t)s->rows * sizeof(int4);
+    p.part_o = (size_t)p.part_rows * D * 4;
+    p.total = p.info + p.part_o + (size_t)p.part_rows * 2 * 4;
     return p;
 }
 
@@ -970,9 +1007,10 @@ extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
         hipLaunchKernelGGL(k_attn_paged_row, dim3(s->rows, H), dim3(64), 0, stream(), a);
         return launch_check("k_attn_paged_row");
     }
-    char* w = (char*)ws;
-    a.info = (int4*)w;
-    w += p.info;
+    a.info = (int4*)ws;
+    a.part_o = (float*)((char*)ws + p.info);
+    a.part_ml = (float*)((char*)a.part_o + p.part_o);
+    a.part_rows = p.part_rows;
     for (int i = 0; i < p.n; i++) {
         const Launch& l = p.l[i];
         if (l.grid > 0x7fffffff) {
@@ -984,15 +1022,13 @@ extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
         a.c_min = l.c_min;
         a.target = l.target;
         a.max_parts = l.max_parts;
-        a.part_o = (float*)w;
-        w += l.part_o;
-        a.part_ml = (float*)w;
-        w += l.part_ml;
+        a.part_row = l.part_row;
         launch(l, a);
         if (launch_check("k_attn_paged")) return -1;
-        if (!l.max_parts) continue;
-        hipLaunchKernelGGL(k_paged_join, dim3(s->rows, H), dim3(kThreads), 0, stream(), a);
-        if (launch_check("k_paged_join")) return -1;
     }
-    return 0;
+    if (!p.part_rows) return 0;
+    // a block a head, or, of many rows, blocks that walk the heads
+    const int gy = s->rows >= 2048 ? 1 : 2048 / s->rows;
+    hipLaunchKernelGGL(k_paged_join, dim3(s->rows, gy < H ? gy : H), dim3(kThreads), 0, stream(), a);
+    return launch_check("k_paged_join");
 }
