@@ -28,104 +28,380 @@ int launch_check(const char* what) {
 }
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxTop = 32;
+constexpr int kWideBlocks = 1024;
+
+// Two launches: k_logprobs_seg reads every logit once, a block a segment of a
+// row held in registers (EPT values a thread), and leaves the segment's
+// maximum, sums, count of tokens before the given one and its first n_top
+// keys in order; k_logprobs_row joins a row's segments.  A row of one segment
+// is done in the first.
+//
+// The first n_top of a segment: a wave finds a value T that at least n_top of
+// its lanes' maxima reach (a binary search over ballots), collects the values
+// from T on (about n_top of them: 24 for 20 of 1024), and the block ranks the
+// waves' few by counting.  Where ties or NaNs make them more than kCand or
+// fewer than needed, the wave takes its largest key n_top times instead.
+constexpr int kCand = 128;                       // collected by a wave
 
 __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0;
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-__device__ __forceinline__ unsigned long long key_of(float x, int i) {
-    return (unsigned long long)order_of(x) << 32 | (uint32_t)~i;
+__device__ __forceinline__ float value_of(uint32_t o) {
+    return o == 0 ? NAN : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ T block_all(T v, T* sh, F f) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = f(v, __shfl_xor(v, o));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) v = f(v, sh[w]);
-    return v;
+#define CGX_DPP_STEP(OP, CTRL, RMASK, IDENT)                                                   \
+    v = OP(v, __builtin_bit_cast(decltype(v), __builtin_amdgcn_update_dpp(                     \
+                  __builtin_bit_cast(int, (decltype(v))(IDENT)), __builtin_bit_cast(int, v), CTRL, RMASK, 0xF, false)))
+#define CGX_DPP_ALL(OP, IDENT)         \
+    CGX_DPP_STEP(OP, 0x111, 0xF, IDENT); \
+    CGX_DPP_STEP(OP, 0x112, 0xF, IDENT); \
+    CGX_DPP_STEP(OP, 0x114, 0xF, IDENT); \
+    CGX_DPP_STEP(OP, 0x118, 0xF, IDENT); \
+    CGX_DPP_STEP(OP, 0x142, 0xA, IDENT); \
+    CGX_DPP_STEP(OP, 0x143, 0xC, IDENT)
+
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ float last(float v) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    CGX_DPP_ALL(fmaxf, -INFINITY);
+    return last(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    CGX_DPP_ALL(add, 0.0f);
+    return last(v);
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    CGX_DPP_ALL(umax, 0u);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// One block a row, one pass for the maximum, one for the sums and the rank,
-// one per alternative.
-__global__ __launch_bounds__(kThreads) void k_logprobs_row(const float* x, size_t ld, int V,
-                                                           const int* tokens, int n_top,
-                                                           float* logprob, int* rank,
-                                                           float* entropy, int* top_tokens,
-                                                           float* top_logprobs) {
-    __shared__ unsigned long long s_u[kWaves];
-    __shared__ double s_d[kWaves];
-    __shared__ float s_f[kWaves];
-    __shared__ int s_i[kWaves];
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const float* row = x + (size_t)r * ld;
-    const int tok = tokens ? tokens[r] : -1;
-    const bool given = tok >= 0 && tok < V;
-    const unsigned long long kt = given ? key_of(row[tok], tok) : 0;
+struct Args {
+    const float* x;
+    size_t ld;
+    int V, nseg, len, n_top;                     // values a segment
+    const int* tokens;
+    float* logprob;
+    int* rank;
+    float* entropy;
+    int* top_tokens;
+    float* top_logprobs;
+    float4* part;                                // [rows][nseg] maximum, sum, weighted sum, count
+    unsigned long long* keys;                    // [rows][nseg][n_top]
+};
+
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));   // rows start anywhere
+
+// What a row's sums say; bad: a NaN or +inf, or nothing above -inf.
+struct Row {
+    double m, z, w;
+    bool bad;
+    float logz, mf;
+};
+__device__ __forceinline__ Row row_of(float m, double z, double w) {
+    Row r;
+    r.m = m;
+    r.z = z;
+    r.w = w;
+    r.bad = !(z > 0.0) || m == INFINITY || m == -INFINITY;
+    r.logz = (float)log(z);
+    r.mf = m;
+    return r;
+}
+__device__ __forceinline__ float lp_of(const Row& r, float v) { return r.bad ? NAN : v - r.mf - r.logz; }
+
+__device__ void write_row(const Args& a, int r, const Row& s, int before) {
+    const int tok = a.tokens ? a.tokens[r] : -1;
+    const bool given = tok >= 0 && tok < a.V;
+    if (a.logprob) a.logprob[r] = given ? lp_of(s, a.x[(size_t)r * a.ld + tok]) : -INFINITY;
+    if (a.rank) a.rank[r] = given ? before : a.V;
+    if (a.entropy) a.entropy[r] = s.bad ? NAN : (float)(log(s.z) - s.w / s.z);
+}
+__device__ __forceinline__ void write_top(const Args& a, int r, const Row& s, int k, unsigned long long key) {
+    a.top_tokens[(size_t)r * a.n_top + k] = key ? (int)~(uint32_t)key : -1;
+    a.top_logprobs[(size_t)r * a.n_top + k] = key ? lp_of(s, value_of((uint32_t)(key >> 32))) : -INFINITY;
+}
+
+template <int EPT>
+__global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
+    __shared__ unsigned long long s_cand[kWaves][kCand], s_top[kMaxTop];
+    __shared__ float s_m[kWaves], s_z[kWaves], s_w[kWaves];
+    __shared__ int s_n[kWaves], s_before[kWaves];
+    const int seg = blockIdx.x % a.nseg, r = blockIdx.x / a.nseg;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* row = a.x + (size_t)r * a.ld;
+    const int begin = seg * a.len, end = min(a.V, begin + a.len);
+    // value (j, c) of a thread is begin + 4 (256 j + tid) + c
+    float v[EPT];
+#pragma unroll
+    for (int j = 0; j < EPT / 4; j++) {
+        const int i = begin + 4 * (kThreads * j + tid);
+        f4 q = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i + 4 <= end) {
+            q = *(const f4*)(row + i);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (i + c < end) q[c] = row[i + c];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[4 * j + c] = q[c];
+    }
+    const int tok = a.tokens ? a.tokens[r] : -1;
+    const bool given = a.rank && tok >= 0 && tok < a.V;
+    const float xt = given ? row[tok] : 0.0f;
+
+    // ---- maximum and sums of the wave
     float m = -INFINITY;
-    int nan = 0, before = 0;
-    for (int i = tid; i < V; i += kThreads) {
-        const float v = row[i];
-        m = fmaxf(m, v);
-        nan |= v != v;
-        before += key_of(v, i) > kt;
+#pragma unroll
+    for (int e = 0; e < EPT; e++) m = fmaxf(m, v[e]);
+    const float lane_max = m;
+    m = wave_max(m);
+    // values past the end are -inf and add nothing; a wave of nothing above
+    // -inf has z = 0, a NaN or +inf makes z NaN
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < EPT; e++) {
+        const float d = v[e] - mu, x = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+        z[e & 3] += x;
+        // below -200 the exponential is 0: the floor keeps -inf from meeting it
+        w[e & 3] = fmaf(fmaxf(d, -200.0f), x, w[e & 3]);
     }
-    m = block_all(m, s_f, [](float p, float q) { return fmaxf(p, q); });
-    nan = block_all(nan, s_i, [](int p, int q) { return p | q; });
-    before = block_all(before, s_i, [](int p, int q) { return p + q; });
-    double z = 0.0, w = 0.0;
-    for (int i = tid; i < V; i += kThreads) {
-        const float d = row[i] - m, e = __expf(d);
-        z += e;
-        if (e > 0.0f) w += (double)(d * e);
-    }
-    z = block_all(z, s_d, [](double p, double q) { return p + q; });
-    w = block_all(w, s_d, [](double p, double q) { return p + q; });
-    const bool bad = nan || m == INFINITY || m == -INFINITY;
-    const float logz = (float)log(z);
-    auto lp = [&](float v) { return bad ? NAN : v - m - logz; };
-    if (tid == 0) {
-        if (logprob) logprob[r] = given ? lp(row[tok]) : -INFINITY;
-        if (rank) rank[r] = given ? before : V;
-        if (entropy) entropy[r] = bad ? NAN : (float)(log(z) - w / z);
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < n_top; k++) {
-        unsigned long long best = 0;
-        for (int i = tid; i < V; i += kThreads) {
-            const unsigned long long u = key_of(row[i], i);
-            if (u < last && u > best) best = u;
-        }
-        best = block_all(best, s_u, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; });
-        last = best;
-        if (tid == 0) {
-            const int at = best ? (int)~(uint32_t)best : -1;
-            top_tokens[(size_t)r * n_top + k] = at;
-            top_logprobs[(size_t)r * n_top + k] = at < 0 ? -INFINITY : lp(row[at]);
+    const float zs = wave_sum((z[0] + z[1]) + (z[2] + z[3])), ws = wave_sum((w[0] + w[1]) + (w[2] + w[3]));
+
+    // ---- tokens before the given one: larger, or equal and of a lower index;
+    //      a NaN comes after every number
+    int before = 0;
+    if (given) {
+        const bool nan = xt != xt;
+#pragma unroll
+        for (int e = 0; e < EPT; e++) {
+            const int i = begin + 4 * (kThreads * (e / 4) + tid) + (e & 3);
+            const bool ahead = nan ? i < end && (v[e] == v[e] || i < tok) : v[e] > xt || (v[e] == xt && i < min(tok, end));
+            before += __popcll(__ballot(ahead));
         }
     }
+
+    // ---- the wave's candidates
+    const int n = a.n_top;
+    if (n) {
+        const uint32_t mine = order_of(lane_max);            // of a lane's numbers: its maximum skips NaN
+        uint32_t lo = 0, hi = wave_umax(mine) + 1;           // lanes reaching lo >= n, reaching hi < n
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int cnt = __popcll(__ballot(mine >= mid));
+            if (cnt >= n) lo = mid; else hi = mid;
+            if (cnt == n) break;
+        }
+        const float T = value_of(lo > 0x007fffffu ? lo : 0x007fffffu);   // -inf at least
+        const int valid = max(0, min(EPT * kThreads, end - begin));
+        int have = 0;
+        if (T > -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < EPT; e++) {
+                const unsigned long long b = __ballot(v[e] >= T);
+                if (b) {
+                    const int at = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+                    const int i = begin + 4 * (kThreads * (e / 4) + tid) + (e & 3);
+                    if (v[e] >= T && at < kCand)
+                        s_cand[wave][at] = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~i;
+                    have += __popcll(b);
+                }
+            }
+        }
+        if (T == -INFINITY || have > kCand || have < n) {
+            // the wave's largest keys one by one
+            have = 0;
+            unsigned long long bound = ~0ull;
+            const int rounds = min(n, valid);
+            while (have < rounds) {
+                unsigned long long best = 0;
+#pragma unroll
+                for (int e = 0; e < EPT; e++) {
+                    const int i = begin + 4 * (kThreads * (e / 4) + tid) + (e & 3);
+                    const unsigned long long k = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~i;
+                    if (i < end && k < bound && k > best) best = k;
+                }
+                for (int o = 1; o < 64; o <<= 1) {
+                    const unsigned long long k = __shfl_xor(best, o);
+                    best = k > best ? k : best;
+                }
+                if (!best) break;                            // the wave has no more values
+                if (lane == 0) s_cand[wave][have] = best;
+                have++;
+                bound = best;
+            }
+        }
+        if (lane == 0) s_n[wave] = have;
+    }
+    if (lane == 0) {
+        s_m[wave] = m;
+        s_z[wave] = zs;
+        s_w[wave] = ws;
+        s_before[wave] = before;
+    }
+    if (tid < kMaxTop) s_top[tid] = 0;
+    __syncthreads();
+    if (n) {
+        // a candidate's place is the number of larger keys, all keys different
+        int cnt[kWaves];
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) cnt[x] = s_n[x];
+#pragma unroll 1
+        for (int c = lane; c < cnt[wave]; c += 64) {
+            const unsigned long long k = s_cand[wave][c];
+            int place = 0;
+            for (int x = 0; x < kWaves; x++)
+                for (int y = 0; y < cnt[x]; y++) place += s_cand[x][y] > k;
+            if (place < n) s_top[place] = k;
+        }
+    }
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWaves; x++) M = fmaxf(M, s_m[x]);
+    double Z = 0.0, W = 0.0;
+    int all = 0;
+#pragma unroll
+    for (int x = 0; x < kWaves; x++) {
+        const bool none = s_m[x] == -INFINITY && s_z[x] == 0.0f;
+        const double d = none ? 0.0 : (double)s_m[x] - (double)M, f = none ? 0.0 : exp(d);
+        Z += f * s_z[x];
+        W += f * (s_w[x] + d * s_z[x]);
+        all += s_before[x];
+    }
+    if (n) __syncthreads();
+    if (a.nseg == 1) {
+        const Row s = row_of(M, Z, W);
+        if (tid == 0) write_row(a, r, s, all);
+        if (tid < n) write_top(a, r, s, tid, s_top[tid]);
+        return;
+    }
+    const size_t at = (size_t)r * a.nseg + seg;
+    if (tid == 0) a.part[at] = make_float4(M, (float)Z, (float)W, __int_as_float(all));
+    if (tid < n) a.keys[at * n + tid] = s_top[tid];
+}
+
+// One wave a row.  Sums: a lane takes every 64th segment.  Keys: a lane a
+// segment's ordered list; the row's next is the largest head, the lowest lane
+// of equal values (segments are in index order).  More than 64 segments come
+// 63 at a time beside the list so far.
+__global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
+    __shared__ unsigned long long s_key[64][kMaxTop + 1];
+    const int r = blockIdx.x, lane = threadIdx.x, n = a.n_top;
+    const float4* part = a.part + (size_t)r * a.nseg;
+    const unsigned long long* keys = a.keys + (size_t)r * a.nseg * n;
+    float M = -INFINITY;
+    for (int s = lane; s < a.nseg; s += 64) M = fmaxf(M, part[s].x);
+    M = wave_max(M);
+    double Z = 0.0, W = 0.0;
+    int before = 0;
+    for (int s = lane; s < a.nseg; s += 64) {
+        const float4 p = part[s];
+        const bool none = p.x == -INFINITY && p.y == 0.0f;
+        const double d = none ? 0.0 : (double)p.x - (double)M, f = none ? 0.0 : exp(d);
+        Z += f * p.y;
+        W += f * (p.z + d * p.y);
+        before += __float_as_int(p.w);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        Z += __shfl_xor(Z, o);
+        W += __shfl_xor(W, o);
+        before += __shfl_xor(before, o);
+    }
+    const Row s = row_of(M, Z, W);
+    if (lane == 0) write_row(a, r, s, before);
+    if (!n) return;
+    unsigned long long out = 0;                  // the row's key number `lane`
+    for (int s0 = 0; s0 < a.nseg;) {
+        const int first = s0 > 0, cnt = min(64 - first, a.nseg - s0);
+        __syncthreads();
+        if (first && lane < n) s_key[0][lane] = out;
+        for (int e = lane; e < cnt * n; e += 64) s_key[first + e / n][e % n] = keys[(size_t)s0 * n + e];
+        __syncthreads();
+        int at = 0;
+        unsigned long long head = lane < first + cnt ? s_key[lane][0] : 0;
+        out = 0;
+        for (int k = 0; k < n; k++) {
+            const uint32_t hi = (uint32_t)(head >> 32);
+            const uint32_t top = wave_umax(hi);
+            // NaN keys have 0 in the high word, as an ended list has: those by their presence
+            const unsigned long long b = __ballot(hi == top && head != 0);
+            if (!b) break;
+            const int win = __builtin_ctzll(b);
+            const unsigned long long key = (unsigned long long)top << 32 |
+                                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)head, win);
+            if (lane == k) out = key;
+            if (lane == win) {
+                at++;
+                head = at < n ? s_key[lane][at] : 0;
+            }
+        }
+        s0 += cnt;
+    }
+    if (lane < n) write_top(a, r, s, lane, out);
+}
+
+// Segments of at most 4096 values (16 a thread) while that gives few blocks,
+// else of 16384: ranking a segment's candidates costs the same for both, but a
+// few rows need the blocks.
+struct Shape {
+    int nseg, len;
+    bool wide;
+};
+Shape shape_of(int rows, int V) {
+    Shape s;
+    const long long wide = ((long long)V + 16383) / 16384;
+    s.wide = wide * rows >= kWideBlocks;
+    const int most = s.wide ? 16384 : 4096;
+    s.nseg = (V + most - 1) / most;
+    s.len = ((V + s.nseg - 1) / s.nseg + 1023) / 1024 * 1024;
+    s.nseg = (V + s.len - 1) / s.len;
+    return s;
 }
 
 }  // namespace
 
 extern "C" size_t cgk_logprobs_ws(int rows, int V, int n_top) {
-    (void)rows;
-    (void)V;
-    (void)n_top;
-    return 0;
+    const Shape s = shape_of(rows, V);
+    return s.nseg == 1 ? 0 : (size_t)rows * s.nseg * (sizeof(float4) + (size_t)n_top * 8);
 }
 
 extern "C" int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens,
                             int n_top, float* logprob, int* rank, float* entropy,
                             int* top_tokens, float* top_logprobs, void* ws) {
-    (void)ws;
-    hipLaunchKernelGGL(k_logprobs_row, dim3(rows), dim3(kThreads), 0, stream(), x, ld, V, tokens,
-                       n_top, logprob, rank, entropy, top_tokens, top_logprobs);
+    const Shape s = shape_of(rows, V);
+    if ((long long)rows * s.nseg > 0x7fffffff) {
+        cgx_set_error("cgx_token_logprobs_dev: too many rows for one call");
+        return -1;
+    }
+    Args a;
+    a.x = x;
+    a.ld = ld;
+    a.V = V;
+    a.nseg = s.nseg;
+    a.len = s.len;
+    a.n_top = n_top;
+    a.tokens = tokens;
+    a.logprob = logprob;
+    a.rank = rank;
+    a.entropy = entropy;
+    a.top_tokens = top_tokens;
+    a.top_logprobs = top_logprobs;
+    a.part = (float4*)ws;
+    a.keys = (unsigned long long*)(a.part + (size_t)rows * s.nseg);
+    const dim3 grid((unsigned)(rows * s.nseg));
+    if (s.wide) hipLaunchKernelGGL(k_logprobs_seg<64>, grid, dim3(kThreads), 0, stream(), a);
+    else hipLaunchKernelGGL(k_logprobs_seg<16>, grid, dim3(kThreads), 0, stream(), a);
+    if (launch_check("k_logprobs_seg")) return -1;
+    if (s.nseg == 1) return 0;
+    hipLaunchKernelGGL(k_logprobs_row, dim3(rows), dim3(64), 0, stream(), a);
     return launch_check("k_logprobs_row");
 }
