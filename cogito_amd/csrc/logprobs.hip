@@ -43,6 +43,7 @@ constexpr int kWideBlocks = 1024;
 // waves' few by counting.  Where ties or NaNs make them more than kCand or
 // fewer than needed, the wave takes its largest key n_top times instead.
 constexpr int kCand = 128;                       // collected by a wave
+constexpr int kRead = 8;                         // keys read at a time in ranking
 
 __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0;
@@ -116,10 +117,14 @@ __device__ __forceinline__ Row row_of(float m, double z, double w) {
 }
 __device__ __forceinline__ float lp_of(const Row& r, float v) { return r.bad ? NAN : v - r.mf - r.logz; }
 
-__device__ void write_row(const Args& a, int r, const Row& s, int before) {
-    const int tok = a.tokens ? a.tokens[r] : -1;
-    const bool given = tok >= 0 && tok < a.V;
-    if (a.logprob) a.logprob[r] = given ? lp_of(s, a.x[(size_t)r * a.ld + tok]) : -INFINITY;
+// The given token's logit, `given` where it is one of the vocabulary.
+__device__ __forceinline__ float given_logit(const Args& a, int r, bool& given, int& tok) {
+    tok = a.tokens ? a.tokens[r] : -1;
+    given = tok >= 0 && tok < a.V;
+    return given ? a.x[(size_t)r * a.ld + tok] : 0.0f;
+}
+__device__ void write_row(const Args& a, int r, const Row& s, int before, bool given, float xt) {
+    if (a.logprob) a.logprob[r] = given ? lp_of(s, xt) : -INFINITY;
     if (a.rank) a.rank[r] = given ? before : a.V;
     if (a.entropy) a.entropy[r] = s.bad ? NAN : (float)(log(s.z) - s.w / s.z);
 }
@@ -130,32 +135,43 @@ __device__ __forceinline__ void write_top(const Args& a, int r, const Row& s, in
 
 template <int EPT>
 __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
-    __shared__ unsigned long long s_cand[kWaves][kCand], s_top[kMaxTop];
+    // collected: bits of the value and the index; ranked: keys
+    __shared__ __attribute__((aligned(16))) unsigned long long s_cand[kWaves][kCand], s_top[kMaxTop];
     __shared__ float s_m[kWaves], s_z[kWaves], s_w[kWaves];
     __shared__ int s_n[kWaves], s_before[kWaves];
     const int seg = blockIdx.x % a.nseg, r = blockIdx.x / a.nseg;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* row = a.x + (size_t)r * a.ld;
-    const int begin = seg * a.len, end = min(a.V, begin + a.len);
+    const int begin = seg * a.len, size = min(a.V - begin, a.len), end = begin + size;
+    int tok;
+    bool given;
+    const float xt = given_logit(a, r, given, tok);
+
     // value (j, c) of a thread is begin + 4 (256 j + tid) + c
     float v[EPT];
+    if (size == EPT * kThreads) {
 #pragma unroll
-    for (int j = 0; j < EPT / 4; j++) {
-        const int i = begin + 4 * (kThreads * j + tid);
-        f4 q = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 4 <= end) {
-            q = *(const f4*)(row + i);
-        } else {
+        for (int j = 0; j < EPT / 4; j++) {
+            const f4 q = *(const f4*)(row + begin + 4 * (kThreads * j + tid));
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (i + c < end) q[c] = row[i + c];
+            for (int c = 0; c < 4; c++) v[4 * j + c] = q[c];
         }
+    } else {
 #pragma unroll
-        for (int c = 0; c < 4; c++) v[4 * j + c] = q[c];
+        for (int j = 0; j < EPT / 4; j++) {
+            const int i = begin + 4 * (kThreads * j + tid);
+            f4 q = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (i + 4 <= end) {
+                q = *(const f4*)(row + i);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (i + c < end) q[c] = row[i + c];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[4 * j + c] = q[c];
+        }
     }
-    const int tok = a.tokens ? a.tokens[r] : -1;
-    const bool given = a.rank && tok >= 0 && tok < a.V;
-    const float xt = given ? row[tok] : 0.0f;
 
     // ---- maximum and sums of the wave
     float m = -INFINITY;
@@ -179,7 +195,16 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
     // ---- tokens before the given one: larger, or equal and of a lower index;
     //      a NaN comes after every number
     int before = 0;
-    if (given) {
+    if (a.rank && given && xt > -INFINITY && (end <= tok || begin > tok)) {
+        // a segment on one side of the token (values past the end count as -inf)
+        if (end <= tok) {
+#pragma unroll
+            for (int e = 0; e < EPT; e++) before += __popcll(__ballot(v[e] >= xt));
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPT; e++) before += __popcll(__ballot(v[e] > xt));
+        }
+    } else if (a.rank && given) {
         const bool nan = xt != xt;
 #pragma unroll
         for (int e = 0; e < EPT; e++) {
@@ -209,18 +234,23 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
                 const unsigned long long b = __ballot(v[e] >= T);
                 if (b) {
                     const int at = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-                    const int i = begin + 4 * (kThreads * (e / 4) + tid) + (e & 3);
                     if (v[e] >= T && at < kCand)
-                        s_cand[wave][at] = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~i;
+                        s_cand[wave][at] = (unsigned long long)__float_as_uint(v[e]) << 32 |
+                                           (uint32_t)(begin + 4 * kThreads * (e / 4) + (e & 3) + 4 * tid);
                     have += __popcll(b);
                 }
+            }
+            // a wave's own LDS words, in order: no barrier
+            for (int c = lane; c < min(have, kCand); c += 64) {
+                const unsigned long long q = s_cand[wave][c];
+                s_cand[wave][c] = (unsigned long long)order_of(__uint_as_float((uint32_t)(q >> 32))) << 32 | (uint32_t)~(uint32_t)q;
             }
         }
         if (T == -INFINITY || have > kCand || have < n) {
             // the wave's largest keys one by one
             have = 0;
             unsigned long long bound = ~0ull;
-            const int rounds = min(n, valid);
+            const int rounds = min(n, size);
             while (have < rounds) {
                 unsigned long long best = 0;
 #pragma unroll
@@ -239,6 +269,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
                 bound = best;
             }
         }
+        // the list's end up to whole reads of the ranking: keys below every other
+        if (lane < kRead && have + lane < kCand) s_cand[wave][have + lane] = 0;
         if (lane == 0) s_n[wave] = have;
     }
     if (lane == 0) {
@@ -258,20 +290,28 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
         for (int c = lane; c < cnt[wave]; c += 64) {
             const unsigned long long k = s_cand[wave][c];
             int place = 0;
+#pragma unroll
             for (int x = 0; x < kWaves; x++)
-                for (int y = 0; y < cnt[x]; y++) place += s_cand[x][y] > k;
+#pragma unroll 1
+                for (int y = 0; y < cnt[x]; y += kRead) {
+                    unsigned long long q[kRead];
+#pragma unroll
+                    for (int i = 0; i < kRead; i++) q[i] = s_cand[x][y + i];
+#pragma unroll
+                    for (int i = 0; i < kRead; i++) place += q[i] > k;
+                }
             if (place < n) s_top[place] = k;
         }
     }
     float M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < kWaves; x++) M = fmaxf(M, s_m[x]);
-    double Z = 0.0, W = 0.0;
+    float Z = 0.0f, W = 0.0f;
     int all = 0;
 #pragma unroll
     for (int x = 0; x < kWaves; x++) {
         const bool none = s_m[x] == -INFINITY && s_z[x] == 0.0f;
-        const double d = none ? 0.0 : (double)s_m[x] - (double)M, f = none ? 0.0 : exp(d);
+        const float d = none ? 0.0f : fmaxf(s_m[x] - M, -200.0f), f = none ? 0.0f : __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
         Z += f * s_z[x];
         W += f * (s_w[x] + d * s_z[x]);
         all += s_before[x];
@@ -279,12 +319,12 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
     if (n) __syncthreads();
     if (a.nseg == 1) {
         const Row s = row_of(M, Z, W);
-        if (tid == 0) write_row(a, r, s, all);
+        if (tid == 0) write_row(a, r, s, all, given, xt);
         if (tid < n) write_top(a, r, s, tid, s_top[tid]);
         return;
     }
     const size_t at = (size_t)r * a.nseg + seg;
-    if (tid == 0) a.part[at] = make_float4(M, (float)Z, (float)W, __int_as_float(all));
+    if (tid == 0) a.part[at] = make_float4(M, Z, W, __int_as_float(all));
     if (tid < n) a.keys[at * n + tid] = s_top[tid];
 }
 
@@ -297,13 +337,22 @@ __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
     const int r = blockIdx.x, lane = threadIdx.x, n = a.n_top;
     const float4* part = a.part + (size_t)r * a.nseg;
     const unsigned long long* keys = a.keys + (size_t)r * a.nseg * n;
-    float M = -INFINITY;
-    for (int s = lane; s < a.nseg; s += 64) M = fmaxf(M, part[s].x);
+    // what the row needs from memory is asked for at once
+    int tok;
+    bool given;
+    const float xt = given_logit(a, r, given, tok);
+    const float4 p0 = lane < a.nseg ? part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    if (lane < a.nseg) {
+#pragma unroll 8
+        for (int k = 0; k < n; k++) s_key[lane][k] = keys[(size_t)lane * n + k];
+    }
+    float M = p0.x;
+    for (int s = lane + 64; s < a.nseg; s += 64) M = fmaxf(M, part[s].x);
     M = wave_max(M);
     double Z = 0.0, W = 0.0;
     int before = 0;
     for (int s = lane; s < a.nseg; s += 64) {
-        const float4 p = part[s];
+        const float4 p = s < 64 ? p0 : part[s];
         const bool none = p.x == -INFINITY && p.y == 0.0f;
         const double d = none ? 0.0 : (double)p.x - (double)M, f = none ? 0.0 : exp(d);
         Z += f * p.y;
@@ -317,17 +366,22 @@ __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
         before += __shfl_xor(before, o);
     }
     const Row s = row_of(M, Z, W);
-    if (lane == 0) write_row(a, r, s, before);
+    if (lane == 0) write_row(a, r, s, before, given, xt);
     if (!n) return;
     unsigned long long out = 0;                  // the row's key number `lane`
     for (int s0 = 0; s0 < a.nseg;) {
         const int first = s0 > 0, cnt = min(64 - first, a.nseg - s0);
+        if (first) {
+            __syncthreads();
+            if (lane < n) s_key[0][lane] = out;
+            if (lane < cnt)
+                for (int k = 0; k < n; k++) s_key[1 + lane][k] = keys[(size_t)(s0 + lane) * n + k];
+        }
         __syncthreads();
-        if (first && lane < n) s_key[0][lane] = out;
-        for (int e = lane; e < cnt * n; e += 64) s_key[first + e / n][e % n] = keys[(size_t)s0 * n + e];
-        __syncthreads();
-        int at = 0;
-        unsigned long long head = lane < first + cnt ? s_key[lane][0] : 0;
+        // the list's next key is read while the one before it is compared
+        int at = 1;
+        const bool mine = lane < first + cnt;
+        unsigned long long head = mine ? s_key[lane][0] : 0, next = mine && n > 1 ? s_key[lane][1] : 0;
         out = 0;
         for (int k = 0; k < n; k++) {
             const uint32_t hi = (uint32_t)(head >> 32);
@@ -340,8 +394,9 @@ __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
                                            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)head, win);
             if (lane == k) out = key;
             if (lane == win) {
+                head = next;
                 at++;
-                head = at < n ? s_key[lane][at] : 0;
+                next = at < n ? s_key[lane][at] : 0;
             }
         }
         s0 += cnt;
@@ -349,21 +404,19 @@ __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
     if (lane < n) write_top(a, r, s, lane, out);
 }
 
-// Segments of at most 4096 values (16 a thread) while that gives few blocks,
-// else of 16384: ranking a segment's candidates costs the same for both, but a
-// few rows need the blocks.
+// Segments of 4096 values (16 a thread) while that gives few blocks, else of
+// 8192: ranking a segment's candidates costs the same for both, but a few
+// rows need the blocks.
 struct Shape {
     int nseg, len;
     bool wide;
 };
 Shape shape_of(int rows, int V) {
     Shape s;
-    const long long wide = ((long long)V + 16383) / 16384;
+    const long long wide = ((long long)V + 8191) / 8192;
     s.wide = wide * rows >= kWideBlocks;
-    const int most = s.wide ? 16384 : 4096;
-    s.nseg = (V + most - 1) / most;
-    s.len = ((V + s.nseg - 1) / s.nseg + 1023) / 1024 * 1024;
-    s.nseg = (V + s.len - 1) / s.len;
+    s.len = s.wide ? 8192 : 4096;
+    s.nseg = (int)(((long long)V + s.len - 1) / s.len);
     return s;
 }
 
@@ -398,7 +451,7 @@ extern "C" int cgk_logprobs(const float* x, size_t ld, int rows, int V, const in
     a.part = (float4*)ws;
     a.keys = (unsigned long long*)(a.part + (size_t)rows * s.nseg);
     const dim3 grid((unsigned)(rows * s.nseg));
-    if (s.wide) hipLaunchKernelGGL(k_logprobs_seg<64>, grid, dim3(kThreads), 0, stream(), a);
+    if (s.wide) hipLaunchKernelGGL(k_logprobs_seg<32>, grid, dim3(kThreads), 0, stream(), a);
     else hipLaunchKernelGGL(k_logprobs_seg<16>, grid, dim3(kThreads), 0, stream(), a);
     if (launch_check("k_logprobs_seg")) return -1;
     if (s.nseg == 1) return 0;
