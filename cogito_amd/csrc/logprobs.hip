@@ -37,11 +37,12 @@ constexpr int kWideBlocks = 1024;
 // keys in order; k_logprobs_row joins a row's segments.  A row of one segment
 // is done in the first.
 //
-// The first n_top of a segment: a wave finds a value T that at least n_top of
-// its lanes' maxima reach (a binary search over ballots), collects the values
-// from T on (about n_top of them: 24 for 20 of 1024), and the block ranks the
-// waves' few by counting.  Where ties or NaNs make them more than kCand or
-// fewer than needed, the wave takes its largest key n_top times instead.
+// The first n_top of a segment: every wave finds the largest value T that at
+// least n_top of the block's 256 lane maxima reach (a binary search over
+// ballots), collects its values from T on (the block together little more than
+// n_top: 22 for 20 of 8192), and the block ranks the few by counting.  Where
+// ties make a wave's more than kCand, or nothing is above -inf, the wave takes
+// its largest key n_top times instead.
 constexpr int kCand = 128;                       // collected by a wave
 constexpr int kRead = 8;                         // keys read at a time in ranking
 
@@ -139,6 +140,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
     __shared__ __attribute__((aligned(16))) unsigned long long s_cand[kWaves][kCand], s_top[kMaxTop];
     __shared__ float s_m[kWaves], s_z[kWaves], s_w[kWaves];
     __shared__ int s_n[kWaves], s_before[kWaves];
+    __shared__ uint32_t s_lane[kThreads];
     const int seg = blockIdx.x % a.nseg, r = blockIdx.x / a.nseg;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* row = a.x + (size_t)r * a.ld;
@@ -217,11 +219,21 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
     // ---- the wave's candidates
     const int n = a.n_top;
     if (n) {
-        const uint32_t mine = order_of(lane_max);            // of a lane's numbers: its maximum skips NaN
-        uint32_t lo = 0, hi = wave_umax(mine) + 1;           // lanes reaching lo >= n, reaching hi < n
+        s_lane[tid] = order_of(lane_max);                    // of a lane's numbers: its maximum skips NaN
+        __syncthreads();
+        uint32_t q[kWaves], hi = 0;
+#pragma unroll
+        for (int x = 0; x < kWaves; x++) {
+            q[x] = s_lane[64 * x + lane];
+            hi = umax(hi, q[x]);
+        }
+        uint32_t lo = 0;                                     // lanes reaching lo: n at least; reaching hi: fewer
+        hi = wave_umax(hi) + 1;
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            const int cnt = __popcll(__ballot(mine >= mid));
+            int cnt = 0;
+#pragma unroll
+            for (int x = 0; x < kWaves; x++) cnt += __popcll(__ballot(q[x] >= mid));
             if (cnt >= n) lo = mid; else hi = mid;
             if (cnt == n) break;
         }
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
                 s_cand[wave][c] = (unsigned long long)order_of(__uint_as_float((uint32_t)(q >> 32))) << 32 | (uint32_t)~(uint32_t)q;
             }
         }
-        if (T == -INFINITY || have > kCand || have < n) {
+        if (T == -INFINITY || have > kCand) {
             // the wave's largest keys one by one
             have = 0;
             unsigned long long bound = ~0ull;
