@@ -401,21 +401,29 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     int base = L - u.n;
     if (a.anc && a.tree_len) base = L - min(max(a.tree_len[b], 0), L);
     if (a.anc) base = max(base, 0);
-    int rq[RT];                                  // the row's entry of the row arrays
-    bool rok[RT];
-    int lim[RT];                                 // last key seen without a bit
-    unsigned long long bits[RT];
-    size_t qrow[RT];
+    // the lane's row of row tile rt, worked out again where it is needed: the
+    // loop over the keys has no registers for it
+    struct RowOf {
+        bool ok;
+        int i, j, t;                             // place in the sequence, head of the KV head, entry of
+                                                 // the row arrays
+        size_t q;                                // row of Q and O
+    };
+    auto row_of = [&](int rt) {
+        int nn = n;
+        asm volatile("" : "+v"(nn));
+        const int r = row0 + 16 * rt + nn;
+        RowOf x;
+        x.ok = r < R;
+        x.i = x.ok ? r / G : 0;
+        x.j = x.ok ? r - x.i * G : 0;
+        x.t = u.r0 + x.i;
+        x.q = (size_t)x.t * a.H + hk * G + x.j;
+        return x;
+    };
     int end = 0;                                 // keys that any of the wave's rows may see
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int r = row0 + 16 * rt + n;
-        rok[rt] = r < R;
-        const int i = rok[rt] ? r / G : 0, h = hk * G + (rok[rt] ? r - i * G : 0);
-        rq[rt] = u.r0 + i;
-        qrow[rt] = (size_t)rq[rt] * a.H + h;
-        lim[rt] = !rok[rt] ? -1 : a.anc ? base - 1 : base + i;
-        bits[rt] = a.anc && rok[rt] ? a.anc[rq[rt]] : 0;
         const int last = min(R - 1, row0 + 16 * rt + 15);
         if (row0 + 16 * rt < R) end = max(end, a.anc ? L : min(L, base + last / G + 1));
     }
@@ -489,13 +497,17 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     float qv[RT][NC][8];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const float* q = a.Q + qrow[rt] * D;
+        const RowOf row = row_of(rt);
+        const float* q = a.Q + row.q * D;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int x = 0; x < 8; x += 4) {
                 const float4 t = *(const float4*)(q + (NG == 1 ? g * (D / 4) + 8 * c : 32 * c + 8 * g) + x);
-                qv[rt][c][x] = t.x; qv[rt][c][x + 1] = t.y; qv[rt][c][x + 2] = t.z; qv[rt][c][x + 3] = t.w;
+                qv[rt][c][x] = row.ok ? t.x : 0.0f;
+                qv[rt][c][x + 1] = row.ok ? t.y : 0.0f;
+                qv[rt][c][x + 2] = row.ok ? t.z : 0.0f;
+                qv[rt][c][x + 3] = row.ok ? t.w : 0.0f;
             }
     }
     constexpr int step = KG * kTile;
@@ -512,7 +524,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                qv[rt][c][i] = rok[rt] ? qv[rt][c][i] * f : 0.0f;
+                qv[rt][c][i] *= f;
                 top = fmaxf(top, fabsf(qv[rt][c][i]));
             }
         top = max_rows(top);
@@ -588,11 +600,14 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
             see[rt] = 0xffu;
             if constexpr (!OPEN) {
                 see[rt] = 0;
+                const RowOf row = row_of(rt);
+                const int lim = !row.ok ? -1 : a.anc ? base - 1 : base + row.i;     // last key seen without a bit
+                const unsigned long long bits = a.anc && row.ok ? a.anc[row.t] : 0;
 #pragma unroll
                 for (int p = 0; p < 8; p++) {
                     const int key = kt + (p < 4 ? 4 * g + p : 12 + 4 * g + p), d = key - base;
-                    const bool bit = key >= base && d < 64 && ((bits[rt] >> (d & 63)) & 1);
-                    const bool yes = key < end && ((td.ok >> (p >> 2)) & 1) && (key <= lim[rt] || bit);
+                    const bool bit = key >= base && d < 64 && ((bits >> (d & 63)) & 1);
+                    const bool yes = key < end && ((td.ok >> (p >> 2)) & 1) && (key <= lim || bit);
                     see[rt] |= (unsigned)yes << p;
                     s[rt][p >> 2][p & 3] = yes ? s[rt][p >> 2][p & 3] : -INFINITY;
                 }
@@ -673,7 +688,18 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     // open tiles first, two in turn: one is loaded while the other is
     // multiplied (past the end page 0's first rows, which nobody looks at);
     // from the first tile on that is not open for all rows, one at a time
+    //
+    // A wave's priority falls as it nears its end: the waves of a SIMD else run
+    // oldest first, and the last one ends alone, with nothing to overlap.
     const int open_to = min(open_end, end) - kTile;
+    const int q2 = k_begin + (end - k_begin) / 2, q1 = (k_begin + q2) / 2, q3 = (q2 + end) / 2;
+    auto pace = [&]() {
+        if (kt >= q3) __builtin_amdgcn_s_setprio(0);
+        else if (kt >= q2) __builtin_amdgcn_s_setprio(1);
+        else if (kt >= q1) __builtin_amdgcn_s_setprio(2);
+        else __builtin_amdgcn_s_setprio(3);
+    };
+    pace();
     if constexpr (NC * NG <= 4) {
         Tile y;
         for (;;) {
@@ -682,6 +708,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
             ahead = pages(kt + 2 * step);
             tile(std::true_type(), x, kt);
             kt += step;
+            pace();
             if (kt > open_to || y.ok != 3) {
                 x = y;
                 break;
@@ -690,6 +717,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
             ahead = pages(kt + 2 * step);
             tile(std::true_type(), y, kt);
             kt += step;
+            pace();
         }
     } else {
         // the words and scales of several groups leave no registers for a
@@ -697,6 +725,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         while (kt <= open_to && x.ok == 3) {
             tile(std::true_type(), x, kt);
             kt += step;
+            pace();
             load(kt, ahead, x);
             ahead = pages(kt + step);
         }
@@ -707,6 +736,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
         load(kt, ahead, x);
         ahead = pages(kt + step);
     }
+    __builtin_amdgcn_s_setprio(0);
 
     // ---- row sums, and O back to one scale relative to m
 #pragma unroll
@@ -781,21 +811,21 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     if (kg) return;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        if (!rok[rt]) continue;
+        const RowOf row = row_of(rt);
+        if (!row.ok) continue;
         if (a.part_rows && u.hk == 0 && u.split == 0 && g == 0) {
             // one of the row's lanes says where its pieces are
-            const int r = row0 + 16 * rt + n, i = r / G;
-            if (r == i * G) {
+            if (row.j == 0) {
                 const long long at = a.part_row + (long long)u.first * TROWS;
-                a.info[2 * (size_t)rq[rt]] = make_int4(u.nsplit, (int)at, (int)(at >> 32), i);
-                a.info[2 * (size_t)rq[rt] + 1] = make_int4(u.tiles, TROWS, 0, 0);
+                a.info[2 * (size_t)row.t] = make_int4(u.nsplit, (int)at, (int)(at >> 32), row.i);
+                a.info[2 * (size_t)row.t + 1] = make_int4(u.tiles, TROWS, 0, 0);
             }
         }
         if (u.part == -1) {
             const float inv = l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f;
-            put(a.O + qrow[rt] * D, o[rt], inv);
+            put(a.O + row.q * D, o[rt], inv);
             if (a.lse && g == 0)
-                a.lse[qrow[rt]] = l[rt] != 0.0f ? 0.69314718055994530942f * (m[rt] + log2f(l[rt])) : -INFINITY;
+                a.lse[row.q] = l[rt] != 0.0f ? 0.69314718055994530942f * (m[rt] + log2f(l[rt])) : -INFINITY;
         } else if (u.part >= 0) {
             const size_t pr = (size_t)a.part_row + (size_t)u.part * TROWS + lr + 16 * rt;
             put(a.part_o + pr * D, o[rt], 1.0f);
@@ -929,7 +959,7 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     // one sequence: one launch, whichever its bound on the rows asks for
     const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
     if (!tiles || both)
-        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, R > 16 ? 512 : 768);
+        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 128, R > 16 ? 448 : 768);
     if (tiles)
         add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 64 + seqs,
             256, 256);
