@@ -15,7 +15,9 @@
 #include "cg_mi355x.h"
 #include "cgx_internal.h"
 
-enum { MAX_SEQS = 4096, MAX_TOP = 32 };
+/* MAX_ROWS: a block of 512 threads a row stays within a launch's 2^32 threads;
+ * MAX_KEYS: positions of a sequence plus a tile's stay within an int */
+enum { MAX_SEQS = 4096, MAX_TOP = 32, MAX_ROWS = 1 << 23, MAX_KEYS = 1 << 30, MAX_VOCAB = 1 << 30 };
 
 static int misaligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
@@ -54,10 +56,10 @@ static int check_cache(const char* who, const cgx_kv_paged_int4* c, int layer) {
 
 /* The sizes of a step, and a table of which page_size positions an entry. */
 static int check_step(const char* who, const cgx_paged_step* s, int page) {
-    if (!s || s->seqs < 1 || s->seqs > MAX_SEQS || s->rows < 0 || s->max_rows < 0 ||
-        s->table_ld < 1 || (long long)s->table_ld * page > INT_MAX) {
-        cgx_set_error("%s: a step of 1..%d sequences, rows, max_rows >= 0 and table_ld >= 1 (below "
-                      "2^31 positions) is required", who, MAX_SEQS);
+    if (!s || s->seqs < 1 || s->seqs > MAX_SEQS || s->rows < 0 || s->rows >= MAX_ROWS ||
+        s->max_rows < 0 || s->table_ld < 1 || (long long)s->table_ld * page > MAX_KEYS) {
+        cgx_set_error("%s: a step of 1..%d sequences, 0..%d rows, max_rows >= 0 and table_ld >= 1 "
+                      "(at most 2^30 positions) is required", who, MAX_SEQS, MAX_ROWS - 1);
         return -1;
     }
     return 0;
@@ -179,8 +181,9 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* c, int layer, const int* sl
                             float* k, float* v) {
     const char* who = "cgx_kv_paged_gather_dev";
     if (check_cache(who, c, layer)) return -1;
-    if (n < 0 || !slots || !k || !v || misaligned(k, 16) || misaligned(v, 16)) {
-        cgx_set_error("%s: slots and 16-byte aligned outputs are required", who);
+    if (n < 0 || n >= MAX_ROWS || !slots || !k || !v || misaligned(k, 16) || misaligned(v, 16)) {
+        cgx_set_error("%s: 0..%d slots and 16-byte aligned outputs are required", who,
+                      MAX_ROWS - 1);
         return -1;
     }
     if (cgx_ensure_init()) return -1;
@@ -188,10 +191,15 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* c, int layer, const int* sl
     return cgk_paged_gather(c, layer, slots, n, k, v);
 }
 
-static int check_heads(const char* who, const cgx_kv_paged_int4* c, int H) {
-    if (H < 1 || H > 65536 || H % c->n_heads) {
+static int check_heads(const char* who, const cgx_kv_paged_int4* c, const cgx_paged_step* s,
+                       int H) {
+    if (H < 1 || H > 65535 || H % c->n_heads) {
         cgx_set_error("%s: %d query heads over %d KV heads (a multiple is required)", who, H,
                       c->n_heads);
+        return -1;
+    }
+    if ((long long)s->rows * H > INT_MAX || !cgk_paged_attention_fits(c, s, H)) {
+        cgx_set_error("%s: %d rows of %d heads are too many for one call", who, s->rows, H);
         return -1;
     }
     return 0;
@@ -201,7 +209,7 @@ size_t cgx_attention_paged_ws(const cgx_kv_paged_int4* c, const cgx_paged_step* 
     const char* who = "cgx_attention_paged_ws";
     if (!c || check_shape(who, c->num_layers, c->num_pages, c->page_size, c->n_heads, c->head_dim,
                           c->group_size) ||
-        check_step(who, s, c->page_size) || check_heads(who, c, H))
+        check_step(who, s, c->page_size) || check_heads(who, c, s, H))
         return 0;
     return cgk_paged_attention_ws(c, s, H);
 }
@@ -211,7 +219,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
                             const int* tree_len, float* O, float* lse, void* ws,
                             size_t ws_bytes) {
     const char* who = "cgx_attention_paged_dev";
-    if (check_cache(who, c, layer) || check_step(who, s, c->page_size) || check_heads(who, c, H))
+    if (check_cache(who, c, layer) || check_step(who, s, c->page_size) || check_heads(who, c, s, H))
         return -1;
     if (!Q || !O || !s->table || !s->row_begin || !s->kv_len || (s->rows && !s->row_seq)) {
         cgx_set_error("%s: Q, O and the step's table, row_begin, row_seq and kv_len are required",
@@ -238,7 +246,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
 }
 
 size_t cgx_token_logprobs_ws(int rows, int V, int n_top) {
-    if (rows < 0 || V < 1 || n_top < 0 || n_top > MAX_TOP) {
+    if (rows < 0 || rows >= MAX_ROWS || V < 1 || V > MAX_VOCAB || n_top < 0 || n_top > MAX_TOP) {
         cgx_set_error("cgx_token_logprobs_ws: invalid argument");
         return 0;
     }
@@ -249,9 +257,10 @@ int cgx_token_logprobs_dev(const float* x, size_t ld, int rows, int V, const int
                            int n_top, float* logprob, int* rank, float* entropy, int* top_tokens,
                            float* top_logprobs, void* ws, size_t ws_bytes) {
     const char* who = "cgx_token_logprobs_dev";
-    if (!x || rows < 0 || V < 1 || ld < (size_t)V || n_top < 0 || n_top > MAX_TOP) {
+    if (!x || rows < 0 || rows >= MAX_ROWS || V < 1 || V > MAX_VOCAB || ld < (size_t)V ||
+        n_top < 0 || n_top > MAX_TOP) {
         cgx_set_error("%s: rows of V >= 1 logits, ld >= V apart, and 0..%d alternatives are "
-                      "required", who, MAX_TOP);
+                      "required (fewer than 2^23 rows, V at most 2^30)", who, MAX_TOP);
         return -1;
     }
     if (!tokens && (logprob || rank)) {

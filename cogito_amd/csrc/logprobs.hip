@@ -443,7 +443,7 @@ extern "C" int cgk_logprobs(const float* x, size_t ld, int rows, int V, const in
                             int n_top, float* logprob, int* rank, float* entropy,
                             int* top_tokens, float* top_logprobs, void* ws) {
     const Shape s = shape_of(rows, V);
-    if ((long long)rows * s.nseg > 0x7fffffff) {
+    if ((long long)rows * s.nseg >= 1 << 24) {      // a launch has fewer than 2^32 threads
         cgx_set_error("cgx_token_logprobs_dev: too many rows for one call");
         return -1;
     }

@@ -57,14 +57,15 @@ struct PagedArgs {
     float* lse;
     // k_attn_paged: sequences of r_lo .. r_hi query rows times heads a KV
     // head, key chunks of at least c_min, about `target` units; partial
-    // results of split tiles (this launch's from row part_row on, at most
-    // max_parts tiles of rows) and where k_paged_join finds those of a row
+    // results of split tiles, this launch's from row part_row on, at most
+    // max_parts tiles of them
     int r_lo, r_hi, c_min, target, max_parts;
     long long part_row, part_rows;
     float* part_o;               // [part_rows][D]
     float* part_ml;              // [part_rows][2]
-    int4* info;                  // [rows] pieces, part_row of the first tile (two words),
-                                 // place among the sequence's rows; then [rows] tiles, tile rows
+    int4* info;                  // [rows][2] where k_paged_join finds a row's pieces: their number,
+                                 // the sequence's first row of part_o (two words), the row's place
+                                 // in the sequence; its tiles, rows a tile, 0, 0
 };
 
 __device__ __forceinline__ float code(unsigned n) { return (float)((int)(n << 28) >> 28); }
@@ -847,8 +848,11 @@ __global__ __launch_bounds__(kThreads) void k_paged_join(PagedArgs a) {
     const int t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int4 f = a.info[2 * (size_t)t], f2 = a.info[2 * (size_t)t + 1];
     const int b = a.row_seq[t], ns = f.x, tiles = f2.x, trows = f2.y, G = a.H / a.Hk, D = a.D;
-    // a row that no sequence has, or of a sequence left out, holds no word of this call
-    if (b < 0 || b >= a.seqs || ns < 2 || tiles < 1 || trows < 1 || f.w < 0) return;
+    if (b < 0 || b >= a.seqs || ns < 2 || tiles < 1 || trows < 1) return;
+    // a row that its sequence does not have, or of a sequence left out, holds
+    // an earlier call's words
+    const int r0 = min(max(a.row_begin[b], 0), a.rows), rn = min(a.row_begin[b + 1], a.rows) - r0;
+    if (f.w != t - r0 || f.w < 0 || f.w >= rn || (long long)rn * G > a.r_hi) return;
     const long long base = (long long)(uint32_t)f.y | (long long)f.z << 32;
     const int d = min(2 * lane, D - 2);
     for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
@@ -1004,6 +1008,15 @@ extern "C" size_t cgk_paged_attention_ws(const cgx_kv_paged_int4* c, const cgx_p
     return plan_of(c, s, H).total;
 }
 
+// whether the blocks stay within a launch's 2^32 threads
+extern "C" int cgk_paged_attention_fits(const cgx_kv_paged_int4* c, const cgx_paged_step* s,
+                                        int H) {
+    const Plan p = plan_of(c, s, H);
+    for (int i = 0; i < p.n; i++)
+        if (p.l[i].grid >= 1 << 23) return 0;
+    return 1;
+}
+
 extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
                                    const cgx_paged_step* s, const float* Q, int H,
                                    const unsigned long long* anc, const int* tree_len, float* O,
@@ -1046,10 +1059,6 @@ extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
     a.part_rows = p.part_rows;
     for (int i = 0; i < p.n; i++) {
         const Launch& l = p.l[i];
-        if (l.grid > 0x7fffffff) {
-            cgx_set_error("cgx_attention_paged_dev: a step of too many rows for one call");
-            return -1;
-        }
         a.r_lo = l.r_lo;
         a.r_hi = l.r_hi;
         a.c_min = l.c_min;

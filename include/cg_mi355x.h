@@ -357,9 +357,9 @@ void cgx_kv_paged_int4_free(cgx_kv_paged_int4* cache);
  * fill it by other means). */
 typedef struct {
     int seqs;             /* sequences, at most 4096 */
-    int rows;             /* entries of the row arrays */
+    int rows;             /* entries of the row arrays, fewer than 2^23 */
     int max_rows;         /* most rows of one sequence (0: any number) */
-    int table_ld;         /* entries of a table row */
+    int table_ld;         /* entries of a table row, at most 2^30 positions */
     const int* kv_old;    /* [seqs] positions whose pages table_old holds */
     const int* kv_keep;   /* [seqs] of those, the positions that stay (NULL: all) */
     const int* rows_new;  /* [seqs] rows that the step adds */
@@ -403,8 +403,8 @@ int cgx_paged_plan_dev(const cgx_paged_step* step, int page_size, int num_pages,
 int cgx_kv_paged_append_dev(cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
                             const float* qkv, int ldq, int H, const float* rope, int rope_rows,
                             float* q_out);
-/* The cached values of n slots: k, v [n][n_heads][head_dim] (0 for a slot
- * outside the cache). */
+/* The cached values of n < 2^23 slots: k, v [n][n_heads][head_dim] (0 for a
+ * slot outside the cache). */
 int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int* slots, int n,
                             float* k, float* v);
 
@@ -418,7 +418,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * Keys of a table entry outside the cache are not seen.  Rows past the last
  * sequence's are left as they were.  Of the step: seqs, rows, max_rows,
  * table_ld, table, row_begin, row_seq and kv_len are read; a sequence of more
- * rows than max_rows (where given) may be left out.
+ * rows than max_rows (where given) may be left out, and its rows as they were.
+ * A call of more than some 2^29 rows times heads is refused.
  * ws: cgx_attention_paged_ws bytes of device memory (16-byte aligned), for
  * this call alone while it runs; every call on the library stream may use
  * the same.  Nothing is allocated: the call may be captured into a graph. */
@@ -427,8 +428,8 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx
                             const float* Q, int H, const unsigned long long* anc,
                             const int* tree_len, float* O, float* lse, void* ws, size_t ws_bytes);
 
-/* Log probabilities of rows of logits x [rows][V] (ld floats apart), device
- * pointers throughout.  For the given token of each row (tokens [rows], NULL:
+/* Log probabilities of rows of logits x [rows][V] (ld floats apart; fewer
+ * than 2^23 rows, V at most 2^30), device pointers throughout.  For the given token of each row (tokens [rows], NULL:
  * none): logprob = x[tok] - log sum exp(x) and rank, the number of tokens
  * before it in the order (value descending, index ascending; NaN last); a
  * token outside [0, V) has -inf and rank V.  entropy: -sum p log p, a token of

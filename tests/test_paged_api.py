@@ -183,3 +183,31 @@ def test_the_reference_plan_keeps_every_page_once():
             continue
         live = np.concatenate([out["table"][b, :R.pages_of(keep[b] + new[b], P)] for b in range(B)])
         assert sorted(np.concatenate([live, out["free"][:out["left"]]]).tolist()) == list(range(pages))
+
+
+def test_sizes_past_a_launch_are_refused(lib):
+    """Row counts, positions and vocabularies whose grids or indices would not fit."""
+    c, s = _cache(), _step()
+    big = _step(rows=2**23)
+    _refused(lib, lib.cgx_paged_plan_dev(C.byref(big), 16, 8, P16, P16 + 512, P16 + 768), "a step of")
+    _refused(lib, lib.cgx_kv_paged_append_dev(C.byref(c), 0, C.byref(big), P16, 512, 4, None, 0, None), "a step of")
+    _refused(lib, lib.cgx_kv_paged_gather_dev(C.byref(c), 0, P16, 2**23, P16, P16), "slots")
+    long = _step(table_ld=2**26 + 1)                       # 16 positions an entry
+    _refused(lib, lib.cgx_attention_paged_dev(C.byref(c), 0, C.byref(long), P16, 2, None, None, P16, None, P16, 1 << 40),
+             "2^30 positions")
+    _refused(lib, lib.cgx_paged_plan_dev(C.byref(long), 16, 8, P16, P16 + 512, P16 + 768), "2^30 positions")
+
+    def attend(cache, step, H):
+        return lib.cgx_attention_paged_dev(C.byref(cache), 0, C.byref(step), P16, H, None, None, P16, None, P16, 1 << 40)
+    _refused(lib, attend(c, s, 65536), "65536 query heads")
+    _refused(lib, attend(c, _step(rows=2**22), 1024), "too many for one call")            # rows times heads
+    _refused(lib, attend(_cache(n_heads=32768), _step(seqs=4096, rows=4096), 32768), "too many for one call")
+    assert lib.cgx_attention_paged_ws(C.byref(c), C.byref(_step(rows=2**22)), 1024) == 0
+    assert "too many" in last_error(lib)
+
+    def logprobs(rows, V):
+        return lib.cgx_token_logprobs_dev(P16, 1 << 31, rows, V, P16, 0, P16, P16, P16, None, None, P16, 1 << 40)
+    _refused(lib, logprobs(2**23, 10), "fewer than 2^23 rows")
+    _refused(lib, logprobs(1, 2**30 + 1), "V at most 2^30")
+    assert lib.cgx_token_logprobs_ws(1, 2**30 + 1, 0) == 0
+    lib.cgx_clear_error()
