@@ -185,6 +185,14 @@ __device__ __forceinline__ float max_rows(float v) {     // over lanes l, l ^ 16
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// the same of the bits of values that are not negative
+__device__ __forceinline__ uint32_t max_bits(float f) {
+    const uint32_t v = __float_as_uint(f);
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t x = max(a[0], a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(b[0], b[1]);
+}
 
 __device__ __forceinline__ float sum_rows(float v) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -193,32 +201,36 @@ __device__ __forceinline__ float sum_rows(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Masks in SGPRs and the fp16 exponent bits in a VGPR, made where the compiler
-// does not see constants: (w & mask) | mag is then one v_and_or_b32 (VOP3 takes
-// no literals here), else two instructions.
+// Masks in SGPRs and the fp16 exponent bits in VGPRs, made where the compiler
+// does not see constants (VOP3 takes no literals here): a nibble's sign bit
+// turned and its exponent set is then one instruction, else two or three.
 struct Nib {
-    uint32_t lo, hi, mag;
+    uint32_t lo, hi, mag_lo, mag_hi;
 };
 __device__ __forceinline__ Nib nib_consts() {
     Nib k;
     asm volatile("s_mov_b32 %0, 0x000f000f" : "=s"(k.lo));
     asm volatile("s_mov_b32 %0, 0x00f000f0" : "=s"(k.hi));
-    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(k.mag));
+    asm volatile("v_mov_b32 %0, 0x64086408" : "=v"(k.mag_lo));
+    asm volatile("v_mov_b32 %0, 0x64806480" : "=v"(k.mag_hi));
     return k;
 }
 
-// Nibbles 0 and 4 (or 1 and 5) of a word of offset-binary codes, exact: 0x6400
-// with a nibble is 1024 + n, or 1024 + 16 n.
+// Nibbles 0 and 4 (or 1 and 5) of a word of codes, exact: 0x6400 with a nibble
+// is 1024 + n, or 1024 + 16 n; with its sign bit turned, 8 more than the code.
+__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t mag) {
+    return __builtin_amdgcn_bitop3_b32(w, mask, mag, 0x6A);      // (w & mask) ^ mag
+}
 __device__ __forceinline__ f16x2 low_nibbles(uint32_t w, const Nib& k) {
     const f16x2 m = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    return __builtin_bit_cast(f16x2, (w & k.lo) | k.mag) + m;
+    return __builtin_bit_cast(f16x2, masked(w, k.lo, k.mag_lo)) + m;
 }
 __device__ __forceinline__ f16x2 high_nibbles(uint32_t w, const Nib& k) {
     const f16x2 s = {(_Float16)0.0625f, (_Float16)0.0625f}, m = {(_Float16)-72.0f, (_Float16)-72.0f};
-    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & k.hi) | k.mag), s, m);
+    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, masked(w, k.hi, k.mag_hi)), s, m);
 }
 
-// Eight offset-binary codes of a word: element p is nibble slot_of(p).
+// Eight codes of a word: element p is nibble slot_of(p).
 __device__ __forceinline__ int slot_of(int p) { return (p >> 1) + 4 * (p & 1); }
 __device__ __forceinline__ f16x8 codes8(uint32_t w, const Nib& k) {
     const f16x2 a = low_nibbles(w, k), b = high_nibbles(w, k), c = low_nibbles(w >> 8, k),
@@ -576,7 +588,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                 for (int rt = 0; rt < RT; rt++) acc[rt] = (f32x4)(0.0f);
 #pragma unroll
                 for (int c = y * NC / NG; c < (y + 1) * NC / NG; c++) {
-                    const f16x8 kc = codes8(td.k[h][c] ^ 0x88888888u, nib);
+                    const f16x8 kc = codes8(td.k[h][c], nib);
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++) {
                         acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, s_q[rg][rt][c][0][ql], acc[rt], 0, 0, 0);
@@ -645,8 +657,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                     w[p] = OPEN || ((see[rt] >> p) & 1) ? pr[rt][p] * vs : 0.0f;
                     big = fmaxf(big, fabsf(w[p]));
                 }
-                big = max_rows(big);
-                const int et = (int)(__float_as_uint(big) >> 23) - 127;
+                const int et = (int)(max_bits(big) >> 23) - 127;
                 const int en = max(max(et, ew[rt][y] - whole[rt]), -100);
                 const float f = __builtin_amdgcn_exp2f((float)(ew[rt][y] - en) - drop[rt]);
                 ew[rt][y] = en;
@@ -656,11 +667,6 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                     for (int t = 0; t < TPG; t++) o[rt][y * TPG + t] *= f;
                 }
             }
-            uint32_t vw[2][NC];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int c = 0; c < NC; c++) vw[h][c] = td.v[h][y][c] ^ 0x88888888u;
 #pragma unroll
             for (int t = 0; t < TPG; t++) {
                 const uint32_t at = (uint32_t)(beta[y] + t / 2) * 0x10001u;
@@ -670,7 +676,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
                 f16x8 va;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const uint32_t (&v)[NC] = vw[h];
+                    const uint32_t (&v)[NC] = td.v[h][y];
                     const uint32_t w01 = __builtin_amdgcn_perm(v[NC > 2 ? 1 : 0], v[0], s01);
                     const uint32_t w23 = __builtin_amdgcn_perm(v[NC > 2 ? b23 + 1 : b23], v[b23], s23);
                     const f16x2 x = t & 1 ? high_nibbles(w01, nib) : low_nibbles(w01, nib);
