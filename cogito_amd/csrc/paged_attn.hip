@@ -70,15 +70,34 @@ struct PagedArgs {
 
 __device__ __forceinline__ float code(unsigned n) { return (float)((int)(n << 28) >> 28); }
 
-// One wave a (row, head), 64 keys a round: scores with a key a lane, then the
-// O update with two dims a lane and byte.
-__global__ __launch_bounds__(64) void k_attn_paged_row(PagedArgs a) {
-    __shared__ float s_q[256];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int b = a.row_seq[t];
-    if (b < 0 || b >= a.seqs) return;
-    const int r0 = a.row_begin[b], n = a.row_begin[b + 1] - r0, i = t - r0;
-    if (i < 0 || i >= n) return;
+// A block a (row, head, piece of the keys), its waves take 64 keys a round in
+// turn: scores with a key a lane (its row of K in 16-byte loads), then O with
+// two dims a lane and byte, the keys' weights and pages from the lanes that
+// have them, eight keys' loads together.  The waves' sums are joined in LDS,
+// those of pieces by k_attn_paged_row_join.  Bound by the latency of a round
+// (about 15 us at 256 dims: a key's 128 bytes are a lane's own, and a byte of V
+// is a load): 5 rows of 8 heads of 256 at 4096 keys 34.5 us, 8 sequences of
+// 1024 keys 22.9 (one wave a row without pieces: 1766 and 445).
+constexpr int kRowWaves = 4, kVKeys = 8;
+
+// the row's sequence and its place there; false: no sequence has it
+__device__ __forceinline__ bool place_of(const PagedArgs& a, int t, int& b, int& n, int& i) {
+    b = a.row_seq[t];
+    if (b < 0 || b >= a.seqs) return false;
+    const int r0 = a.row_begin[b];
+    n = a.row_begin[b + 1] - r0;
+    i = t - r0;
+    return i >= 0 && i < n;
+}
+
+__global__ __launch_bounds__(64 * kRowWaves) void k_attn_paged_row(PagedArgs a) {
+    constexpr int W = kRowWaves;
+    __shared__ __attribute__((aligned(16))) float s_q[256];
+    __shared__ float s_ml[W][2], s_o[W][256];
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int b, n, i;
+    if (!place_of(a, t, b, n, i)) return;
     const int D = a.D, half = D / 2, gs = a.gs, ng = D / gs, cb = D / 32;
     const int L = (int)min((long long)max(a.kv_len[b], 0), (long long)a.table_ld << a.lp);
     const int hk = h / (a.H / a.Hk);
@@ -92,30 +111,67 @@ __global__ __launch_bounds__(64) void k_attn_paged_row(PagedArgs a) {
         end = min(L, max(0, L - n + i + 1));
         base = end;
     }
+    const int S = gridDim.z, piece = ((end + S - 1) / S + 63) / 64 * 64, from = blockIdx.z * piece;
+    end = min(end, from + piece);
     const float* q = a.Q + ((size_t)t * a.H + h) * D;
-    for (int d = lane; d < D; d += 64) s_q[d] = q[d] * a.scale;
+    for (int d = threadIdx.x; d < D; d += 64 * W) s_q[d] = q[d] * a.scale;
     __syncthreads();
 
+    // the lane's dims d, d + 1 (and of D > 128, those 128 later) in a V block
+    int voff[2], vg[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int d = min(2 * (lane + 64 * x), D - 2), nb = d / (D / 16);
+        voff[x] = nb * 16 * cb + (d - nb * (D / 16)) / 2;
+        vg[x] = d / gs;
+    }
     float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < end; k0 += 64) {
+    for (int k0 = from + 64 * wave; k0 < end; k0 += 64 * W) {
         const int j = k0 + lane;
         bool see = j < end && (j < base || (j - base < 64 && ((bits >> (j - base)) & 1)));
         int page = -1;
         if (see) page = a.table[(size_t)b * a.table_ld + (j >> a.lp)];
         see = see && page >= 0 && page < a.num_pages;
-        const size_t ph = (size_t)(see ? page : 0) * a.Hk + hk;
-        const int at = j & ((1 << a.lp) - 1);
-        const size_t pr = (ph << a.lp) + at;
+        // the page's head: of 2^31 of them K alone would have 2^39 bytes
+        const int ph = (see ? page : 0) * a.Hk + hk;
+        const size_t pr = ((size_t)ph << a.lp) + (j & ((1 << a.lp) - 1));
         float s = -INFINITY;
         if (see) {
+            const u32x4* kw = (const u32x4*)(a.kp + pr * half);
+            const float* ks = a.ks + pr * ng;
+            float sc = *ks;
+            int left = gs;
             s = 0.0f;
-            for (int g = 0; g < ng; g++) {
-                float dot = 0.0f;
-                for (int d = g * gs; d < (g + 1) * gs; d += 2) {
-                    const unsigned c = a.kp[pr * half + d / 2];
-                    dot += s_q[d] * code(c & 15) + s_q[d + 1] * code(c >> 4);
+            for (int w = 0; w < cb; w++) {
+                const u32x4 x = kw[w];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const f32x4 q0 = *(const f32x4*)(s_q + 32 * w + 8 * c), q1 = *(const f32x4*)(s_q + 32 * w + 8 * c + 4);
+                    float d[4];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const f32x4& qq = y < 2 ? q0 : q1;
+                        d[y] = qq[2 * y & 3] * code(x[c] >> (8 * y)) + qq[(2 * y & 3) + 1] * code(x[c] >> (8 * y + 4));
+                    }
+                    if (gs % 8 == 0) {
+                        s += ((d[0] + d[1]) + (d[2] + d[3])) * sc;
+                        left -= 8;
+                        if (!left && 32 * w + 8 * c + 8 < D) {
+                            sc = *++ks;
+                            left = gs;
+                        }
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            s += d[y] * sc;
+                            left -= 2;
+                            if (!left && 32 * w + 8 * c + 2 * y + 2 < D) {
+                                sc = *++ks;
+                                left = gs;
+                            }
+                        }
+                    }
                 }
-                s += dot * a.ks[pr * ng + g];
             }
         }
         float top = s;
@@ -129,35 +185,85 @@ __global__ __launch_bounds__(64) void k_attn_paged_row(PagedArgs a) {
         l = l * f + sum;
         m = mn;
         for (int x = 0; x < 4; x++) o[x] *= f;
-        const int nk = min(64, end - k0);
-        for (int kk = 0; kk < nk; kk++) {
-            const float w = __shfl(p, kk);
-            const size_t pk = (size_t)__shfl((long long)ph, kk);
-            if (w == 0.0f) continue;
-            const int ak = (k0 + kk) & ((1 << a.lp) - 1);
+        // a key that is not seen has weight 0 and page 0: read, not added
+        for (int kk = 0; kk < min(64, end - k0); kk += kVKeys) {
+            uint32_t c[kVKeys][2];
+            float v[kVKeys][2], w[kVKeys];
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int d = 2 * (lane + 64 * x);
-                if (d >= D) break;
-                const int nb = d / (D / 16);
-                const unsigned c = a.vp[(pk << a.lp) * half +
-                                        ((size_t)(ak >> 4) * 16 + nb) * (16 * cb) +
-                                        (size_t)(ak & 15) * cb + (d - nb * (D / 16)) / 2];
-                const float sv = w * a.vs[((pk << a.lp) + ak) * ng + d / gs];
-                o[2 * x] += sv * code(c & 15);
-                o[2 * x + 1] += sv * code(c >> 4);
+            for (int y = 0; y < kVKeys; y++) {
+                w[y] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), kk + y));
+                const size_t pk = (size_t)__builtin_amdgcn_readlane(ph, kk + y) << a.lp;
+                const int ak = (k0 + kk + y) & ((1 << a.lp) - 1);
+                const uint8_t* vp = a.vp + pk * half + (size_t)(ak >> 4) * (256 * cb) + (ak & 15) * cb;
+                const float* vs = a.vs + (pk + ak) * ng;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    c[y][x] = vp[voff[x]];
+                    v[y][x] = vs[vg[x]];
+                }
             }
+#pragma unroll
+            for (int y = 0; y < kVKeys; y++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float sv = w[y] == 0.0f ? 0.0f : w[y] * v[y][x];
+                    o[2 * x] += sv * code(c[y][x] & 15);
+                    o[2 * x + 1] += sv * code(c[y][x] >> 4);
+                }
         }
     }
-    float* out = a.O + ((size_t)t * a.H + h) * D;
+    if (lane == 0) {
+        s_ml[wave][0] = m;
+        s_ml[wave][1] = l;
+    }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const int d = 2 * (lane + 64 * x);
-        if (d >= D) break;
-        out[d] = l != 0.0f ? o[2 * x] / l : 0.0f;
-        out[d + 1] = l != 0.0f ? o[2 * x + 1] / l : 0.0f;
+        if (d < D) *(f32x2*)&s_o[wave][d] = (f32x2){o[2 * x], o[2 * x + 1]};
     }
-    if (a.lse && lane == 0) a.lse[(size_t)t * a.H + h] = l != 0.0f ? m + logf(l) : -INFINITY;
+    __syncthreads();
+    float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) M = fmaxf(M, s_ml[w][0]);
+    float f[W];
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        f[w] = s_ml[w][0] == M ? 1.0f : __expf(s_ml[w][0] - M);
+        sum += f[w] * s_ml[w][1];
+    }
+    const size_t row = (size_t)t * a.H + h, pr = row * S + blockIdx.z;
+    for (int d = threadIdx.x; d < D; d += 64 * W) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) v += f[w] * s_o[w][d];
+        if (S > 1) a.part_o[pr * D + d] = v;
+        else a.O[row * D + d] = sum != 0.0f ? v / sum : 0.0f;
+    }
+    if (threadIdx.x) return;
+    if (S > 1) *(f32x2*)(a.part_ml + 2 * pr) = (f32x2){M, sum};
+    else if (a.lse) a.lse[row] = sum != 0.0f ? M + logf(sum) : -INFINITY;
+}
+
+// Joins the S <= 64 pieces of a (row, head): one wave, four dims a lane.
+__global__ __launch_bounds__(64) void k_attn_paged_row_join(PagedArgs a, int S) {
+    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, D = a.D;
+    int b, n, i;
+    if (!place_of(a, t, b, n, i)) return;
+    const size_t row = (size_t)t * a.H + h, pr = row * S;
+    const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (pr + min(lane, S - 1)));
+    float M = ml.x;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+    const float w = ml.x == M ? 1.0f : __expf(ml.x - M);
+    float l = lane < S ? w * ml.y : 0.0f;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+    const int d = min(4 * lane, D - 4);
+    f32x4 o = (f32x4)(0.0f);
+#pragma unroll 4
+    for (int s = 0; s < S; s++) o += __shfl(w, s) * *(const f32x4*)(a.part_o + (pr + s) * D + d);
+    if (4 * lane < D) *(f32x4*)(a.O + row * D + d) = l != 0.0f ? o / l : (f32x4)(0.0f);
+    if (a.lse && lane == 0) a.lse[row] = l != 0.0f ? M + logf(l) : -INFINITY;
 }
 
 // ------------------------------------------------------- matrix-core kernel
@@ -932,6 +1038,7 @@ struct Launch {
 };
 struct Plan {
     bool fast;
+    int row_pieces;              // not fast: pieces of the keys
     Launch l[2];
     int n;
     long long part_rows;
@@ -939,12 +1046,24 @@ struct Plan {
 };
 
 constexpr int kSplitRows = 32;
+// Blocks up to which k_attn_paged_row's keys are cut: 5 rows of 8 heads of 256
+// at 4096 keys take 46 us with 512, 34.5 with 1024 and 2048, and 239 uncut.
+constexpr int kRowBlocks = 1024;
 
 Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     Plan p = {};
     const int D = c->head_dim, G = H / c->n_heads;
     p.fast = D <= 128 && c->group_size % 32 == 0;
-    if (!p.fast || !s->rows) return p;
+    if (!s->rows) return p;
+    if (!p.fast) {
+        const long long blocks = (long long)s->rows * H;
+        const long long keys = ((long long)s->table_ld * c->page_size + 64 * kRowWaves - 1) / (64 * kRowWaves);
+        long long n = blocks < kRowBlocks ? kRowBlocks / blocks : 1;
+        if (n > keys) n = keys;
+        p.row_pieces = (int)(n > 64 ? 64 : n);
+        if (n > 1) p.total = (size_t)blocks * p.row_pieces * (D + 2) * 4;
+        return p;
+    }
     const long long most = s->max_rows && s->max_rows < s->rows ? s->max_rows : s->rows;
     const long long R = most * G, seqs = s->seqs < s->rows ? s->seqs : s->rows;
     const long long keys = (long long)s->table_ld * c->page_size;
@@ -1056,8 +1175,13 @@ extern "C" int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer,
     a.lse = lse;
     const Plan p = plan_of(c, s, H);
     if (!p.fast) {
-        hipLaunchKernelGGL(k_attn_paged_row, dim3(s->rows, H), dim3(64), 0, stream(), a);
-        return launch_check("k_attn_paged_row");
+        a.part_o = (float*)ws;
+        a.part_ml = a.part_o + (size_t)s->rows * H * p.row_pieces * a.D;
+        hipLaunchKernelGGL(k_attn_paged_row, dim3(s->rows, H, p.row_pieces), dim3(64 * kRowWaves), 0, stream(), a);
+        if (launch_check("k_attn_paged_row")) return -1;
+        if (p.row_pieces == 1) return 0;
+        hipLaunchKernelGGL(k_attn_paged_row_join, dim3(s->rows, H), dim3(64), 0, stream(), a, p.row_pieces);
+        return launch_check("k_attn_paged_row_join");
     }
     a.info = (int4*)ws;
     a.part_o = (float*)((char*)ws + p.info);

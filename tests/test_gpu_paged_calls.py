@@ -167,3 +167,20 @@ def test_logprob_graphs_share_a_workspace(gpu):
             for a, b in zip(bits(s), f):
                 np.testing.assert_array_equal(a, b)
     assert gpu.cgx_graph_free(g) == 0
+
+
+@pytest.mark.parametrize("H,Hk,D,gs", [(4, 2, 256, 256), (2, 2, 192, 24), (3, 1, 64, 16)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_rows_of_other_heads_over_long_keys(gpu, H, Hk, D, gs, tree):
+    """Head sizes and scale groups off the matrix cores: keys cut over blocks, pieces without keys, rows without."""
+    rng = np.random.default_rng(D + gs)
+    b = R.Batch(gpu, rng, [3000, 5, 0, 257], [3, 2, 1, 9], 16, H, Hk, D, gs, pad=2).bind()
+    anc = [int(x) for x in rng.integers(0, 1 << 9, b.T)] if tree else None
+    ref, got = b.reference(anc=anc), b.attend(anc=anc)
+    n = int(b.begin[-1])
+    _near(got[0], ref, slice(0, n))
+    fin = np.isfinite(ref[1][:n])
+    np.testing.assert_array_equal(got[1][:n][~fin], ref[1][:n][~fin])
+    g, e = got[1][:n][fin], ref[1][:n][fin]
+    assert np.all(np.abs(g - e) <= TOL * (1 + np.abs(e)))
+    assert np.all(got[0][n:] == 7.0) and np.all(got[1][n:] == 7.0)
