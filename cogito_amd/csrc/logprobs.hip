@@ -43,6 +43,10 @@ constexpr int kWideBlocks = 1024;
 // n_top: 22 for 20 of 8192), and the block ranks the few by counting.  Where
 // ties make a wave's more than kCand, or nothing is above -inf, the wave takes
 // its largest key n_top times instead.
+//
+// Bound by the logits' bytes: 301 rows of 128256 with 20 alternatives 37 us
+// (4.1 TB/s); 5 rows of 32000 by latency, 6.6 us.  A threshold a wave took 4 us
+// more, 64 values a thread 31 more.
 constexpr int kCand = 128;                       // collected by a wave
 constexpr int kRead = 8;                         // keys read at a time in ranking
 
@@ -343,7 +347,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
 // One wave a row.  Sums: a lane takes every 64th segment.  Keys: a lane a
 // segment's ordered list; the row's next is the largest head, the lowest lane
 // of equal values (segments are in index order).  More than 64 segments come
-// 63 at a time beside the list so far.
+// 63 at a time beside the list so far.  Bound by latency, n_top dependent steps
+// among others: 7.5 us for 301 rows of 16 segments and 20 keys, 3.7 for 5.
 __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
     __shared__ unsigned long long s_key[64][kMaxTop + 1];
     const int r = blockIdx.x, lane = threadIdx.x, n = a.n_top;
@@ -417,8 +422,10 @@ __global__ __launch_bounds__(64) void k_logprobs_row(Args a) {
 }
 
 // Segments of 4096 values (16 a thread) while that gives few blocks, else of
-// 8192: ranking a segment's candidates costs the same for both, but a few
-// rows need the blocks.
+// 8192: ranking a segment's candidates costs the same for both, but a few rows
+// need the blocks (5 rows of 32000: 11.2 and 12.8 us; 301 of 128256: 53 and
+// 43).  A row of 8192 or less is one segment, and needs no second launch (7.7
+// us of two, 6.5 of one).
 struct Shape {
     int nseg, len;
     bool wide;
@@ -426,7 +433,7 @@ struct Shape {
 Shape shape_of(int rows, int V) {
     Shape s;
     const long long wide = ((long long)V + 8191) / 8192;
-    s.wide = wide * rows >= kWideBlocks;
+    s.wide = wide * rows >= kWideBlocks || (V > 4096 && V <= 8192);
     s.len = s.wide ? 8192 : 4096;
     s.nseg = (int)(((long long)V + s.len - 1) / s.len);
     return s;

@@ -42,8 +42,8 @@ int launch_check(const char* what) {
 // rows, its table entries, its pages given back.  No block waits for another
 // and nothing is read that another block writes, which one launch needs; the
 // scan costs each block less than a second launch would.  Bound by latency:
-// lengths, table and stack are three dependent loads, 4 us against 2.5 for an
-// empty launch.
+// lengths, table and stack are three dependent loads.  64 sequences of up to 5
+// rows take 4.4 us, 256 prompts of up to 381 rows 4.2, an empty launch 2.5.
 constexpr int kPlanThreads = 256, kPlanWaves = kPlanThreads / 64;
 
 struct PlanArgs {
@@ -238,7 +238,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
 // from where a thread packs eight neighbouring values of a head.  Row,
 // slot and values are asked for together, then the rotary words.  Bound by
 // latency for few rows (two dependent loads), then by bytes: (H + 2 Hk) D in,
-// H D out a row, the packed row is a sixteenth of that.
+// H D out a row, the packed row is a sixteenth of that.  5 rows of 32/8 heads
+// of 128 take 4.0 us, 64 sequences of up to 5 rows 5.0, 2039 rows of 12/12
+// heads of 64 11.9 (2.2 TB/s: a block has one round of loads, which nothing
+// of its own overlaps).
 constexpr int kAppThreads = 256;
 
 struct AppendArgs {
@@ -403,7 +406,8 @@ __device__ __forceinline__ float2 code_pair(uint32_t b) {
     return make_float2((float)((int)(b << 28) >> 28), (float)((int)(b << 24) >> 28));
 }
 
-// Four dims of K and of V a thread.
+// Four dims of K and of V a thread: bound by latency (a slot, then its bytes
+// and scales), 3.0 us for 5 rows, 6.0 for 2039 rows of 12 heads of 64.
 __global__ __launch_bounds__(256) void k_paged_gather(const uint8_t* kp, const uint8_t* vp,
                                                       const float* ks, const float* vs, int lp,
                                                       int Hk, int D, int gs, int num_slots,

@@ -282,6 +282,16 @@ __global__ __launch_bounds__(64) void k_attn_paged_row_join(PagedArgs a, int S) 
 // The exponent follows the weights' largest of the tile, or what the sums so
 // far still need (e minus the whole part of the maximum's rise): V scales may
 // lie any distance apart.
+//
+// Bound, for one row a sequence, by the pages' bytes and the kernel's ends (64
+// sequences of up to 4096 keys, 32/8 heads of 128: 51 us, the tiles 27 to 36 of
+// them at 6 TB/s, search, first loads and operands 5, sums 3, join 6); for many
+// rows by vector issue beside the products (509 rows after 2048 keys: 61 us, 9
+// vector instructions a product: codes to fp16, softmax, hi + lo); for few rows
+// by the chain of dependent steps (5 rows at 4096 keys: 17 us, tiles 5.5).
+// Pieces of all items in even lengths (63 us instead of 54), the scores of the
+// next tile beside the softmax (56 and 64 us), long pieces first (no change)
+// and more than one round of blocks (57) were slower or no faster.
 constexpr int kTile = 32;                        // keys of a wave's step
 
 __device__ __forceinline__ float max_rows(float v) {     // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -952,7 +962,8 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
 // Joins the pieces of split rows: block = (row, every gridDim.y-th head), its
 // waves take pieces in turn; m relative to the largest of the pieces, as in
 // the block itself.  A row's place comes in one load, its pieces' sums and
-// values together in the next.
+// values together in the next.  Bound by those two and its launch: 3.6 us for 5
+// rows of 32 heads, 6 to 8 for 64 and for 95 pieces of one row.
 constexpr int kJoin = 4;                         // pieces a wave loads at a time
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_paged_join(PagedArgs a) {
@@ -1045,6 +1056,9 @@ struct Plan {
     size_t info, part_o, total;
 };
 
+// Up to 32 rows times heads a KV head are one unit whose waves share the keys;
+// with 16 the draft trees take 43 us instead of 29 and 5 rows of 4 heads each
+// at 4096 keys 21 instead of 17.
 constexpr int kSplitRows = 32;
 // Blocks up to which k_attn_paged_row's keys are cut: 5 rows of 8 heads of 256
 // at 4096 keys take 46 us with 512, 34.5 with 1024 and 2048, and 239 uncut.
@@ -1087,7 +1101,8 @@ Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     };
     // Smallest chunks: a cut has to save more than the launch that joins its
     // pieces (4-5 us).  Mean of 40 mixed batches: 128 and 256 keys 18.4 us, 384
-    // and 512 17.8, 384 and 768 18.2.
+    // and 512 17.8, 384 and 768 18.2.  The units fill the card once (3, 2 and 1
+    // blocks a CU): with a third more 64 sequences take 57 us instead of 51.
     // One sequence: one launch, whichever its bound on the rows asks for
     const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
     if (!tiles || both)
