@@ -184,3 +184,17 @@ def test_rows_of_other_heads_over_long_keys(gpu, H, Hk, D, gs, tree):
     g, e = got[1][:n][fin], ref[1][:n][fin]
     assert np.all(np.abs(g - e) <= TOL * (1 + np.abs(e)))
     assert np.all(got[0][n:] == 7.0) and np.all(got[1][n:] == 7.0)
+
+
+def test_the_most_sequences(gpu):
+    """4096 sequences, 64 a lane of the search, most of a key or two and some without rows or keys."""
+    rng = np.random.default_rng(24)
+    kv = [int(k) for k in rng.integers(0, 4, 4096)]
+    rows = [int(min(k, r)) for k, r in zip(kv, rng.integers(0, 3, 4096))]
+    for i, (k, n) in {0: (900, 1), 777: (40, 33), 2048: (2000, 3), 4095: (70, 20)}.items():
+        kv[i], rows[i] = k, n
+    b = R.Batch(gpu, rng, kv, rows, 16, 2, 1, 32, 32, pad=3).bind()
+    ref, (o, _) = b.reference(), b.attend()
+    n = int(b.begin[-1])
+    _near(o, ref, slice(0, n))
+    assert np.all(o[n:] == 7.0)

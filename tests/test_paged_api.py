@@ -16,7 +16,7 @@ P16 = (C.addressof(_BUF) + 15) & ~15
 
 def _cache(**kw):
     c = CgxKvPagedInt4(num_layers=2, num_pages=8, page_size=16, n_heads=2, head_dim=64, group_size=64)
-    c.k_pages, c.v_pages, c.k_scales, c.v_scales = P16, P16 + 1024, P16 + 2048, P16 + 3072
+    c.k_pages, c.v_pages, c.k_scales, c.v_scales = P16, P16 + 1024, P16 + 2048, P16 + 4096
     for k, v in kw.items():
         setattr(c, k, v)
     return c
@@ -162,7 +162,7 @@ def test_logprob_arguments(lib):
 
 
 def test_the_reference_plan_keeps_every_page_once():
-    """The checker itself: pages are conserved, and a refused step leaves everything."""
+    """The reference plan itself: pages are conserved, and a refused step leaves everything."""
     rng = np.random.default_rng(0)
     for _ in range(50):
         B, P, ld = int(rng.integers(1, 9)), 16, 6
