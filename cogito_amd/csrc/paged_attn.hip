@@ -689,11 +689,10 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     }
 
     // OPEN: every key of the tile is seen by every row; NR: row tiles that hold
-    // rows.  A unit of 32 rows that has 16 or fewer (a rest, or a sequence of few
-    // rows beside ones of many) leaves the second one out: draft trees 27.8 us
-    // instead of 28.9, 40 mixed batches 17.4 instead of 17.8.
-    constexpr bool HALF = RT == 2 && RG == 1;
-    const bool two = R - u.tile * TROWS > 16;
+    // rows.  A wave that has 16 rows or fewer (a rest, or a sequence of few rows
+    // beside ones of many) leaves the second one out: draft trees 27.8 us instead
+    // of 28.9, 40 mixed batches 17.4 instead of 17.8.
+    const bool two = R - row0 > 16;
     auto tile_of = [&](auto open, auto row_tiles, const Tile& td, int kt) {
         constexpr bool OPEN = decltype(open)::value;
         constexpr int NR = decltype(row_tiles)::value;
@@ -814,7 +813,7 @@ __global__ __launch_bounds__(64 * RG * KG, WPS) void k_attn_paged(PagedArgs a) {
     };
 
     auto tile = [&](auto open, const Tile& td, int kt) {
-        if constexpr (HALF) {
+        if constexpr (RT == 2) {
             if (!two) return tile_of(open, std::integral_constant<int, 1>(), td, kt);
         }
         tile_of(open, std::integral_constant<int, RT>(), td, kt);
@@ -1070,7 +1069,7 @@ struct Plan {
 };
 
 // Up to 32 rows times heads a KV head are one unit whose waves share the keys;
-// with 16 the draft trees take 43 us instead of 29 and 5 rows of 4 heads each
+// with 16 the draft trees take 43 us instead of 28 and 5 rows of 4 heads each
 // at 4096 keys 21 instead of 17.
 constexpr int kSplitRows = 32;
 // Blocks up to which k_attn_paged_row's keys are cut: 5 rows of 8 heads of 256
