@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64) void k_attn_paged_row_join(PagedArgs a, int S) 
 // Bound, for one row a sequence, by the pages' bytes and the kernel's ends (64
 // sequences of up to 4096 keys, 32/8 heads of 128: 51 us, the tiles 27 to 36 of
 // them at 6 TB/s, search, first loads and operands 5, sums 3, join 6); for many
-// rows by vector issue beside the products (509 rows after 2048 keys: 61 us, 9
+// rows by vector issue beside the products (509 rows after 2048 keys: 62 us, 9
 // vector instructions a product: codes to fp16, softmax, hi + lo); for few rows
 // by the chain of dependent steps (5 rows at 4096 keys: 17 us, tiles 5.5).
 // Pieces of all items in even lengths (63 us instead of 54), the scores of the
