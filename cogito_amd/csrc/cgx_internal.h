@@ -282,7 +282,8 @@ int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer, const cgx_paged_s
                         const float* Q, int H, const unsigned long long* anc,
                         const int* tree_len, float* O, float* lse, void* ws);
 /* Token log probabilities (logprobs.hip). */
-size_t cgk_logprobs_ws(int rows, int V, int n_top);
+size_t cgk_logprobs_ws(int rows, int V, int n_top);      /* of any call up to these sizes */
+size_t cgk_logprobs_need(int rows, int V, int n_top);    /* of this one */
 int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens, int n_top,
                  float* logprob, int* rank, float* entropy, int* top_tokens,
                  float* top_logprobs, void* ws);

@@ -271,7 +271,7 @@ int cgx_token_logprobs_dev(const float* x, size_t ld, int rows, int V, const int
         cgx_set_error("%s: top_tokens and top_logprobs go with n_top > 0", who);
         return -1;
     }
-    const size_t need = cgk_logprobs_ws(rows, V, n_top);
+    const size_t need = cgk_logprobs_need(rows, V, n_top);
     if (need && (!ws || misaligned(ws, 16) || ws_bytes < need)) {
         cgx_set_error("%s: a 16-byte aligned workspace of %zu bytes is required (%zu given)", who,
                       need, ws ? ws_bytes : (size_t)0);

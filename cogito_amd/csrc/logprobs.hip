@@ -441,9 +441,21 @@ Shape shape_of(int rows, int V) {
 
 }  // namespace
 
-extern "C" size_t cgk_logprobs_ws(int rows, int V, int n_top) {
+// What a call with these sizes writes.
+extern "C" size_t cgk_logprobs_need(int rows, int V, int n_top) {
     const Shape s = shape_of(rows, V);
     return s.nseg == 1 ? 0 : (size_t)rows * s.nseg * (sizeof(float4) + (size_t)n_top * 8);
+}
+
+// What no call of at most these sizes passes.  Segments of 4096 values are
+// taken while those of 8192 number fewer than kWideBlocks, so they number at
+// most 2 kWideBlocks - 2 of a call: the bound below holds for either length,
+// and rises with rows and V where the segments' number itself falls.
+extern "C" size_t cgk_logprobs_ws(int rows, int V, int n_top) {
+    if (V <= 8192) return 0;
+    const size_t narrow = (size_t)rows * (((size_t)V + 4095) / 4096), wide = (size_t)rows * (((size_t)V + 8191) / 8192);
+    const size_t most = wide > 2 * kWideBlocks - 2 ? wide : 2 * kWideBlocks - 2;
+    return (narrow < most ? narrow : most) * (sizeof(float4) + (size_t)n_top * 8);
 }
 
 extern "C" int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens,

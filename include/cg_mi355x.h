@@ -438,7 +438,8 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx
  * NaN or +inf, or nothing above -inf, has NaN for every log probability
  * within V and for its entropy.  NULL outputs are left out (top_tokens and
  * top_logprobs go together).  ws: cgx_token_logprobs_ws bytes of device memory
- * (16-byte aligned), as for cgx_attention_paged_dev. */
+ * (16-byte aligned), as for cgx_attention_paged_dev: enough for every call of
+ * at most these rows, V and n_top. */
 size_t cgx_token_logprobs_ws(int rows, int V, int n_top);
 int cgx_token_logprobs_dev(const float* logits, size_t ld, int rows, int V, const int* tokens,
                            int n_top, float* logprob, int* rank, float* entropy,
