@@ -277,7 +277,9 @@ int cgk_paged_append(const cgx_kv_paged_int4* c, int layer, const cgx_paged_step
 int cgk_paged_gather(const cgx_kv_paged_int4* c, int layer, const int* slots, int n, float* k,
                      float* v);
 int cgk_paged_attention_fits(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H);
+/* workspace of any call up to these sizes, and of this one */
 size_t cgk_paged_attention_ws(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H);
+size_t cgk_paged_attention_need(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H);
 int cgk_paged_attention(const cgx_kv_paged_int4* c, int layer, const cgx_paged_step* s,
                         const float* Q, int H, const unsigned long long* anc,
                         const int* tree_len, float* O, float* lse, void* ws);

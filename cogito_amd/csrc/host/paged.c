@@ -234,7 +234,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
         cgx_set_error("%s: Q and O have to be 16-byte aligned", who);
         return -1;
     }
-    const size_t need = cgk_paged_attention_ws(c, s, H);
+    const size_t need = cgk_paged_attention_need(c, s, H);
     if (need && (!ws || misaligned(ws, 16) || ws_bytes < need)) {
         cgx_set_error("%s: a 16-byte aligned workspace of %zu bytes is required (%zu given)", who,
                       need, ws ? ws_bytes : (size_t)0);

@@ -1076,52 +1076,80 @@ constexpr int kSplitRows = 32;
 // at 4096 keys take 46 us with 512, 34.5 with 1024 and 2048, and 239 uncut.
 constexpr int kRowBlocks = 1024;
 
+// What the host knows of a step.
+struct Sizes {
+    bool fast;
+    long long R, seqs, keys;     // rows times heads a KV head of one sequence, sequences, positions
+    long long tiles;             // of 64 rows
+    int row_keys;                // pieces that k_attn_paged_row's keys can be cut into
+};
+Sizes sizes_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
+    const int G = H / c->n_heads;
+    const long long most = s->max_rows && s->max_rows < s->rows ? s->max_rows : s->rows;
+    Sizes z;
+    z.fast = c->head_dim <= 128 && c->group_size % 32 == 0;
+    z.R = most * G;
+    z.seqs = s->seqs < s->rows ? s->seqs : s->rows;
+    z.keys = (long long)s->table_ld * c->page_size;
+    z.tiles = ((long long)s->rows * G) / 64 + z.seqs;
+    const long long n = (z.keys + 64 * kRowWaves - 1) / (64 * kRowWaves);
+    z.row_keys = (int)(n > 64 ? 64 : n);
+    return z;
+}
+
+// How finely the keys of a launch's tiles are cut, and the blocks and split
+// tiles that follow.
+struct Cut {
+    int trows, c_min, target;
+    long long grid(long long tiles, int heads, long long keys) const {
+        // round(len / C) pieces: at most target units by length and one a tile
+        const long long whole = tiles * heads, pieces = (keys + c_min / 2) / c_min, cut = whole * (pieces < 1 ? 1 : pieces);
+        const long long g = whole + target + 8;      // 8: C is rounded in 32 bits
+        return g > cut ? cut : g;
+    }
+    int parts(long long tiles, int heads, long long keys) const {
+        if ((keys + c_min / 2) / c_min < 2) return 0;
+        // a split tile has at least 1.5 C keys, so at most 4/3 target pieces in all
+        const long long g = grid(tiles, heads, keys), most = target * 4 / 3 + 8;
+        return (int)(g < most ? g : most);
+    }
+};
+// Smallest chunks: a cut has to save more than the launch that joins its
+// pieces (4-5 us).  Mean of 40 mixed batches: 128 and 256 keys 18.4 us, 384
+// and 512 17.8, 384 and 768 18.2.  The units fill the card once (3, 2 and 1
+// blocks a CU): with a third more 64 sequences take 57 us instead of 51.
+constexpr Cut kCut16 = {16, 384, 768}, kCut32 = {32, 384, 448}, kCut64 = {64, 512, 256};
+
 Plan plan_of(const cgx_kv_paged_int4* c, const cgx_paged_step* s, int H) {
     Plan p = {};
-    const int D = c->head_dim, G = H / c->n_heads;
-    p.fast = D <= 128 && c->group_size % 32 == 0;
+    const Sizes z = sizes_of(c, s, H);
+    const int D = c->head_dim;
+    p.fast = z.fast;
     if (!s->rows) return p;
     if (!p.fast) {
         const long long blocks = (long long)s->rows * H;
-        const long long keys = ((long long)s->table_ld * c->page_size + 64 * kRowWaves - 1) / (64 * kRowWaves);
-        long long n = blocks < kRowBlocks ? kRowBlocks / blocks : 1;
-        if (n > keys) n = keys;
-        p.row_pieces = (int)(n > 64 ? 64 : n);
-        if (n > 1) p.total = (size_t)blocks * p.row_pieces * (D + 2) * 4;
+        const long long n = blocks < kRowBlocks ? kRowBlocks / blocks : 1;
+        p.row_pieces = (int)(n < z.row_keys ? n : z.row_keys);
+        if (p.row_pieces > 1) p.total = (size_t)blocks * p.row_pieces * (D + 2) * 4;
         return p;
     }
-    const long long most = s->max_rows && s->max_rows < s->rows ? s->max_rows : s->rows;
-    const long long R = most * G, seqs = s->seqs < s->rows ? s->seqs : s->rows;
-    const long long keys = (long long)s->table_ld * c->page_size;
-    auto add = [&](int rt, bool ks, int lo, long long hi, long long tiles, int c_min, int target) {
+    auto add = [&](int rt, int lo, long long hi, long long tiles, const Cut& cut) {
         Launch& l = p.l[p.n++];
-        const int trows = 16 * rt * (ks ? 1 : 2);
-        l.rt = ks ? rt : -rt;
+        l.rt = rt;
         l.r_lo = lo;
         l.r_hi = (int)(hi > 0x7fffffff ? 0x7fffffff : hi);
-        l.c_min = c_min;
-        l.target = target;
-        // round(len / C) pieces: at most target units by length and one a tile
-        const long long whole = tiles * c->n_heads, pieces = (keys + c_min / 2) / c_min;
-        l.grid = whole + target + 8;             // 8: C is rounded in 32 bits
-        if (l.grid > whole * (pieces < 1 ? 1 : pieces)) l.grid = whole * (pieces < 1 ? 1 : pieces);
-        // a split tile has at least 1.5 C keys, so at most 4/3 target pieces in all
-        l.max_parts = pieces > 1 ? target * 4 / 3 + 8 : 0;
-        if (l.max_parts > l.grid) l.max_parts = (int)l.grid;
+        l.c_min = cut.c_min;
+        l.target = cut.target;
+        l.grid = cut.grid(tiles, c->n_heads, z.keys);
+        l.max_parts = cut.parts(tiles, c->n_heads, z.keys);
         l.part_row = p.part_rows;
-        p.part_rows += (long long)l.max_parts * trows;
+        p.part_rows += (long long)l.max_parts * cut.trows;
     };
-    // Smallest chunks: a cut has to save more than the launch that joins its
-    // pieces (4-5 us).  Mean of 40 mixed batches: 128 and 256 keys 18.4 us, 384
-    // and 512 17.8, 384 and 768 18.2.  The units fill the card once (3, 2 and 1
-    // blocks a CU): with a third more 64 sequences take 57 us instead of 51.
     // One sequence: one launch, whichever its bound on the rows asks for
-    const bool tiles = R > kSplitRows, both = tiles && s->seqs > 1;
+    const bool tiles = z.R > kSplitRows, both = tiles && s->seqs > 1;
     if (!tiles || both)
-        add(R > 16 ? 2 : 1, true, 1, R < kSplitRows ? R : kSplitRows, seqs, 384, R > 16 ? 448 : 768);
-    if (tiles)
-        add(2, false, both ? kSplitRows + 1 : 1, 0x7fffffff, ((long long)s->rows * G) / 64 + seqs,
-            512, 256);
+        add(z.R > 16 ? 2 : 1, 1, z.R < kSplitRows ? z.R : kSplitRows, z.seqs, z.R > 16 ? kCut32 : kCut16);
+    if (tiles) add(-2, both ? kSplitRows + 1 : 1, 0x7fffffff, z.tiles, kCut64);
     if (!p.part_rows) return p;
     p.info = 2 * (size_t)s->rows * sizeof(int4);
     p.part_o = (size_t)p.part_rows * D * 4;
@@ -1155,9 +1183,31 @@ void launch(const Launch& l, const PagedArgs& a) {
 
 }  // namespace
 
+// What this call writes.
+extern "C" size_t cgk_paged_attention_need(const cgx_kv_paged_int4* c, const cgx_paged_step* s,
+                                           int H) {
+    return plan_of(c, s, H).total;
+}
+
+// What no call of at most these sequences, rows, positions and rows of one
+// sequence passes: fewer rows may be cut into more pieces, or take launches
+// that the step itself does not need.
 extern "C" size_t cgk_paged_attention_ws(const cgx_kv_paged_int4* c, const cgx_paged_step* s,
                                          int H) {
-    return plan_of(c, s, H).total;
+    const Sizes z = sizes_of(c, s, H);
+    const size_t word = (size_t)(c->head_dim + 2) * 4;           // a partial row
+    if (!s->rows) return 0;
+    if (!z.fast) {
+        if (z.row_keys < 2 || 2 * H > kRowBlocks) return 0;
+        const long long cut = (long long)s->rows * H * z.row_keys;
+        return (size_t)(cut < kRowBlocks ? cut : kRowBlocks) * word;
+    }
+    auto rows_of = [&](const Cut& cut, long long tiles) { return (long long)cut.parts(tiles, c->n_heads, z.keys) * cut.trows; };
+    const long long few = rows_of(kCut16, z.seqs), some = z.R > 16 ? rows_of(kCut32, z.seqs) : 0,
+                    many = z.R > kSplitRows ? rows_of(kCut64, z.tiles) : 0;
+    long long most = s->seqs > 1 ? some + many : some > many ? some : many;
+    if (most < few) most = few;
+    return most ? 2 * (size_t)s->rows * sizeof(int4) + (size_t)most * word : 0;
 }
 
 // whether the blocks stay within a launch's 2^32 threads

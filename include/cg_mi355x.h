@@ -422,7 +422,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * A call of more than some 2^29 rows times heads is refused.
  * ws: cgx_attention_paged_ws bytes of device memory (16-byte aligned), for
  * this call alone while it runs; every call on the library stream may use
- * the same.  Nothing is allocated: the call may be captured into a graph. */
+ * the same.  The size is enough for every call with the same heads and at most
+ * these seqs, rows, table_ld and max_rows (0 being the largest).  Nothing is allocated: the call may be captured into a graph. */
 size_t cgx_attention_paged_ws(const cgx_kv_paged_int4* cache, const cgx_paged_step* step, int H);
 int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
                             const float* Q, int H, const unsigned long long* anc,
