@@ -9,6 +9,9 @@ import pytest
 
 from cogito_amd.capi import CgxKvPagedInt4, CgxPagedStep, last_error
 
+_BUF = C.create_string_buffer(256)
+P16 = (C.addressof(_BUF) + 15) & ~15                       # never read: the calls are refused first
+
 # either side of every bound on the rows that the choice of segments has
 ROWS = sorted({r + d for r in (1, 2, 8, 9, 16, 32, 63, 64, 128, 255, 256, 342, 512, 1000, 1024, 4096)
                for d in (-1, 0, 1)} - {0})
@@ -65,3 +68,31 @@ def test_attention_workspaces_grow_with_the_step(lib, shape, H):
         for seqs in (1, 2, 64):
             need = _sizes(lib, shape, [300], [dict(seqs=seqs, rows=rows, max_rows=m) for m in (1, 2, 4, 5, 8, 9, 17, 33, 400, 0)], H)
             assert need == sorted(need), (rows, seqs)
+
+
+@pytest.mark.parametrize("shape,H,kw", [
+    (dict(n_heads=2, head_dim=64, group_size=64), 4, dict(seqs=2, rows=4, max_rows=1)),        # a split launch
+    (dict(n_heads=2, head_dim=64, group_size=64), 64, dict(seqs=1, rows=4)),                   # tiles of 64 rows
+    (dict(n_heads=2, head_dim=256, group_size=256), 4, dict(seqs=2, rows=4))])                 # off the matrix cores
+def test_attention_refuses_other_workspaces(lib, shape, H, kw):
+    c = CgxKvPagedInt4(num_layers=1, num_pages=64, page_size=16, **shape)
+    c.k_pages, c.v_pages, c.k_scales, c.v_scales = P16, P16, P16, P16
+    s = CgxPagedStep(table_ld=256, **kw)
+    s.table, s.row_begin, s.row_seq, s.kv_len = P16, P16, P16, P16
+    need = lib.cgx_attention_paged_ws(C.byref(c), C.byref(s), H)
+    assert need > 0, last_error(lib)
+    for ws, n in ((P16, need - 1), (P16, 0), (None, need), (P16 + 4, need), (None, 0)):
+        assert lib.cgx_attention_paged_dev(C.byref(c), 0, C.byref(s), P16, H, None, None, P16, None, ws, n) == -1
+        assert "workspace of" in last_error(lib)
+        lib.cgx_clear_error()
+
+
+@pytest.mark.parametrize("rows,V,n_top", [(2, 9000, 3), (5, 32000, 0), (4096, 12000, 20)])
+def test_logprobs_refuse_other_workspaces(lib, rows, V, n_top):
+    top = P16 if n_top else None
+    need = lib.cgx_token_logprobs_ws(rows, V, n_top)
+    assert need > 0
+    for ws, n in ((P16, need - 1), (P16, 0), (None, need), (P16 + 8, need), (None, 0)):
+        assert lib.cgx_token_logprobs_dev(P16, V, rows, V, P16, n_top, P16, P16, P16, top, top, ws, n) == -1
+        assert "workspace of" in last_error(lib)
+        lib.cgx_clear_error()
