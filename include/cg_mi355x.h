@@ -398,8 +398,9 @@ int cgx_paged_plan_dev(const cgx_paged_step* step, int page_size, int num_pages,
  * (cgx_rope_table_dev from position 0; NULL: no rotation), queries stored to
  * q_out [rows][H][head_dim] (NULL: not stored), keys and values quantised by
  * cg_kv_cache_int4_append's rule, bit for bit.  Rows with a slot outside the
- * cache, or a position outside rope, are skipped; two rows of one slot leave
- * either's values. */
+ * cache, or a position outside rope, are skipped (their rows of q_out too).  A
+ * slot given to two rows holds no value of either: its codes and scales are a
+ * mix of both rows' (the plan gives no slot twice). */
 int cgx_kv_paged_append_dev(cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
                             const float* qkv, int ldq, int H, const float* rope, int rope_rows,
                             float* q_out);
