@@ -321,8 +321,8 @@ int cgx_attention_int4_kv_batch_dev(const float* Q, int B, int Nq, int H,
                                     float* O);
 
 /* -------------------------------- paged INT4 KV cache and serving steps */
-/* A KV cache in pages of page_size positions that any number of sequences
- * share (no counterpart in the reference, whose cache holds one sequence).
+/* A KV cache in pages of page_size positions, one pool for any number of
+ * sequences (no counterpart in the reference, whose cache holds one sequence).
  * All four arrays live in HBM; values and scales are those of
  * cg_kv_cache_int4 (codes [-8, 7], scale = absmax / 7 per group), laid out
  * per layer for the attention's lanes:
@@ -377,7 +377,9 @@ typedef struct {
  * keeps kv_keep[b] of its kv_old[b] positions and adds rows_new[b] rows.  A
  * page past the last position goes back on the stack free_pages[0 ..
  * *free_count), sequence by sequence; then new pages are taken from its top
- * down, sequence by sequence.  *free_left receives the new count (a word of
+ * down, sequence by sequence.  A page has one holder, a table entry or the
+ * stack; nothing counts holders, so one that two sequences have would go back
+ * twice.  *free_left receives the new count (a word of
  * its own, so that a step can be planned again); entries of the stack below
  * *free_count are not written, the stack holds num_pages entries.  Table
  * entries past a sequence's pages are left as they were in place, -1 in
