@@ -230,6 +230,11 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
         cgx_set_error("%s: tree_len without ancestor bits", who);
         return -1;
     }
+    if (anc && !tree_len && s->max_rows > 64 && s->rows > 64) {
+        cgx_set_error("%s: ancestor bits of sequences of more than 64 rows (max_rows %d) need "
+                      "tree_len", who, s->max_rows);
+        return -1;
+    }
     if (misaligned(Q, 16) || misaligned(O, 16) || misaligned(anc, 8)) {
         cgx_set_error("%s: Q and O have to be 16-byte aligned", who);
         return -1;

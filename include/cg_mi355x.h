@@ -416,8 +416,11 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * 1/sqrt(head_dim), lse [rows][H] (natural logarithm; NULL: none).  Row i of
  * sequence b sees keys up to kv_len[b] - (rows of b) + i; with anc (device,
  * [rows] ancestor bits), every key below kv_len[b] - w and those keys
- * kv_len[b] - w + j, j < w, whose bit j is set, w = tree_len[b] (at most 64;
- * tree_len NULL: the rows of b).  A row that sees nothing gets 0 (lse -inf).
+ * kv_len[b] - w + j, j < w, whose bit j is set, w = tree_len[b] (tree_len NULL:
+ * the rows of b).  A row has 64 bits: of a longer window no row sees the keys
+ * from the 65th on, so w is at most 64, and a step whose max_rows allows more
+ * is refused without tree_len (a prompt chunk goes in a step of its own, without
+ * anc).  A row that sees nothing gets 0 (lse -inf).
  * Keys of a table entry outside the cache are not seen.  Rows past the last
  * sequence's are left as they were.  Of the step: seqs, rows, max_rows,
  * table_ld, table, row_begin, row_seq and kv_len are read; a sequence of more
@@ -426,7 +429,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * ws: cgx_attention_paged_ws bytes of device memory (16-byte aligned), for
  * this call alone while it runs; every call on the library stream may use
  * the same.  The size is enough for every call with the same heads and at most
- * these seqs, rows, table_ld and max_rows (0 being the largest).  Nothing is allocated: the call may be captured into a graph. */
+ * these seqs, rows, table_ld and max_rows (0 being the largest).  Nothing is
+ * allocated: the call may be captured into a graph. */
 size_t cgx_attention_paged_ws(const cgx_kv_paged_int4* cache, const cgx_paged_step* step, int H);
 int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
                             const float* Q, int H, const unsigned long long* anc,
