@@ -33,6 +33,7 @@ def test_logprob_workspaces_grow_with_the_call(lib, n_top):
 def _sizes(lib, shape, table_lds, steps, H):
     cache = CgxKvPagedInt4(num_layers=1, num_pages=64, page_size=16, **shape)
     out = []
+    lib.cgx_clear_error()
     for ld in table_lds:
         for kw in steps:
             s = CgxPagedStep(table_ld=ld, **kw)
