@@ -54,6 +54,27 @@ static int check_cache(const char* who, const cgx_kv_paged_int4* c, int layer) {
     return 0;
 }
 
+/* Memory of a call: blocks read inputs while others write outputs, so that an
+ * output may lie over nothing else.  The first, an output, may be span `place`
+ * (-1: none) where both start alike. */
+typedef struct {
+    const void* p;
+    size_t n;        /* bytes */
+    int out;
+} span;
+static int check_spans(const char* who, const span* s, int n, int place) {
+    for (int i = 0; i < n; i++)
+        for (int j = 0; s[i].out && j < n; j++) {
+            const uintptr_t a = (uintptr_t)s[i].p, b = (uintptr_t)s[j].p;
+            if (i == j || !a || !b || !s[i].n || !s[j].n || (!i && j == place && a == b)) continue;
+            if (a < b + s[j].n && b < a + s[i].n) {
+                cgx_set_error("%s: an output or the workspace overlaps another argument", who);
+                return -1;
+            }
+        }
+    return 0;
+}
+
 /* The sizes of a step, and a table of which page_size positions an entry. */
 static int check_step(const char* who, const cgx_paged_step* s, int page) {
     if (!s || s->seqs < 1 || s->seqs > MAX_SEQS || s->rows < 0 || s->rows >= MAX_ROWS ||
@@ -172,6 +193,15 @@ int cgx_kv_paged_append_dev(cgx_kv_paged_int4* c, int layer, const cgx_paged_ste
                       who);
         return -1;
     }
+    const size_t T = (size_t)s->rows, D = (size_t)c->head_dim;
+    const span mem[] = {
+        {q_out, T * H * D * 4, 1},
+        {qkv, T ? ((T - 1) * ldq + (H + 2 * (size_t)c->n_heads) * D) * 4 : 0, 0},
+        {rope, (size_t)(rope ? rope_rows : 0) * D * 4, 0},
+        {s->row_slot, T * 4, 0},
+        {rope ? s->row_pos : NULL, T * 4, 0}};
+    /* one row may be rotated in its place: a thread's values are its own */
+    if (check_spans(who, mem, 5, T == 1 ? 1 : -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!s->rows) return 0;
     return cgk_paged_append(c, layer, s, qkv, ldq, H, rope, rope_rows, q_out);
@@ -186,6 +216,9 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* c, int layer, const int* sl
                       MAX_ROWS - 1);
         return -1;
     }
+    const size_t bytes = (size_t)n * c->n_heads * c->head_dim * 4;
+    const span mem[] = {{k, bytes, 1}, {v, bytes, 1}, {slots, (size_t)n * 4, 0}};
+    if (check_spans(who, mem, 3, -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!n) return 0;
     return cgk_paged_gather(c, layer, slots, n, k, v);
@@ -245,6 +278,19 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
                       need, ws ? ws_bytes : (size_t)0);
         return -1;
     }
+    const size_t T = (size_t)s->rows, B = (size_t)s->seqs;
+    const span mem[] = {{O, T * H * c->head_dim * 4, 1},
+                        {lse, T * H * 4, 1},
+                        {ws, need, 1},
+                        {Q, T * H * c->head_dim * 4, 0},
+                        {s->table, B * s->table_ld * 4, 0},
+                        {s->row_begin, (B + 1) * 4, 0},
+                        {s->row_seq, T * 4, 0},
+                        {s->kv_len, B * 4, 0},
+                        {anc, T * 8, 0},
+                        {tree_len, B * 4, 0}};
+    /* O in the place of Q: a block writes the rows and heads that it has read */
+    if (check_spans(who, mem, 10, 3)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!s->rows) return 0;
     return cgk_paged_attention(c, layer, s, Q, H, anc, tree_len, O, lse, ws);
@@ -282,6 +328,16 @@ int cgx_token_logprobs_dev(const float* x, size_t ld, int rows, int V, const int
                       need, ws ? ws_bytes : (size_t)0);
         return -1;
     }
+    const size_t T = (size_t)rows;
+    const span mem[] = {{logprob, T * 4, 1},
+                        {rank, T * 4, 1},
+                        {entropy, T * 4, 1},
+                        {top_tokens, T * n_top * 4, 1},
+                        {top_logprobs, T * n_top * 4, 1},
+                        {ws, need, 1},
+                        {x, T ? ((T - 1) * ld + V) * 4 : 0, 0},
+                        {tokens, T * 4, 0}};
+    if (check_spans(who, mem, 8, -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!rows) return 0;
     return cgk_logprobs(x, ld, rows, V, tokens, n_top, logprob, rank, entropy, top_tokens,

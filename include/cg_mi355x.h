@@ -402,12 +402,13 @@ int cgx_paged_plan_dev(const cgx_paged_step* step, int page_size, int num_pages,
  * cg_kv_cache_int4_append's rule, bit for bit.  Rows with a slot outside the
  * cache, or a position outside rope, are skipped (their rows of q_out too).  A
  * slot given to two rows holds no value of either: its codes and scales are a
- * mix of both rows' (the plan gives no slot twice). */
+ * mix of both rows' (the plan gives no slot twice).  q_out may overlap no input
+ * (a call of one row may rotate it in its place, q_out = qkv). */
 int cgx_kv_paged_append_dev(cgx_kv_paged_int4* cache, int layer, const cgx_paged_step* step,
                             const float* qkv, int ldq, int H, const float* rope, int rope_rows,
                             float* q_out);
 /* The cached values of n < 2^23 slots: k, v [n][n_heads][head_dim] (0 for a
- * slot outside the cache). */
+ * slot outside the cache), apart from each other and from slots. */
 int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int* slots, int n,
                             float* k, float* v);
 
@@ -425,7 +426,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * sequence's are left as they were.  Of the step: seqs, rows, max_rows,
  * table_ld, table, row_begin, row_seq and kv_len are read; a sequence of more
  * rows than max_rows (where given) may be left out, and its rows as they were.
- * A call of more than some 2^29 rows times heads is refused.
+ * A call of more than some 2^29 rows times heads is refused, and one whose
+ * outputs or workspace overlap another argument (O = Q excepted).
  * ws: cgx_attention_paged_ws bytes of device memory (16-byte aligned), for
  * this call alone while it runs; every call on the library stream may use
  * the same.  The size is enough for every call with the same heads and at most
@@ -445,7 +447,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx
  * n_top (at most 32) of that order, past V -1 and -inf.  A row that holds a
  * NaN or +inf, or nothing above -inf, has NaN for every log probability
  * within V and for its entropy.  NULL outputs are left out (top_tokens and
- * top_logprobs go together).  ws: cgx_token_logprobs_ws bytes of device memory
+ * top_logprobs go together); no output may overlap another argument.  ws: cgx_token_logprobs_ws bytes of device memory
  * (16-byte aligned), as for cgx_attention_paged_dev: enough for every call of
  * at most these rows, V and n_top. */
 size_t cgx_token_logprobs_ws(int rows, int V, int n_top);
