@@ -242,7 +242,6 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_seg(Args a) {
             if (cnt == n) break;
         }
         const float T = value_of(lo > 0x007fffffu ? lo : 0x007fffffu);   // -inf at least
-        const int valid = max(0, min(EPT * kThreads, end - begin));
         int have = 0;
         if (T > -INFINITY) {
 #pragma unroll

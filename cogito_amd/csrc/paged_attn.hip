@@ -260,7 +260,6 @@ __global__ __launch_bounds__(64) void k_attn_paged_row_join(PagedArgs a, int S) 
     for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
     const int d = min(4 * lane, D - 4);
     f32x4 o = (f32x4)(0.0f);
-#pragma unroll 4
     for (int s = 0; s < S; s++) o += __shfl(w, s) * *(const f32x4*)(a.part_o + (pr + s) * D + d);
     if (4 * lane < D) *(f32x4*)(a.O + row * D + d) = l != 0.0f ? o / l : (f32x4)(0.0f);
     if (a.lse && lane == 0) a.lse[row] = l != 0.0f ? M + logf(l) : -INFINITY;
