@@ -422,7 +422,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* cache, int layer, const int
  * from the 65th on, so w is at most 64, and a step whose max_rows allows more
  * is refused without tree_len (a prompt chunk goes in a step of its own, without
  * anc).  A row that sees nothing gets 0 (lse -inf).
- * Keys of a table entry outside the cache are not seen.  Rows past the last
+ * Keys of a table entry outside the cache are not seen.  K scales are taken up
+ * to 2^100.  Rows past the last
  * sequence's are left as they were.  Of the step: seqs, rows, max_rows,
  * table_ld, table, row_begin, row_seq and kv_len are read; a sequence of more
  * rows than max_rows (where given) may be left out, and its rows as they were.
@@ -439,15 +440,16 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx
                             const int* tree_len, float* O, float* lse, void* ws, size_t ws_bytes);
 
 /* Log probabilities of rows of logits x [rows][V] (ld floats apart; fewer
- * than 2^23 rows, V at most 2^30), device pointers throughout.  For the given token of each row (tokens [rows], NULL:
- * none): logprob = x[tok] - log sum exp(x) and rank, the number of tokens
- * before it in the order (value descending, index ascending; NaN last); a
- * token outside [0, V) has -inf and rank V.  entropy: -sum p log p, a token of
- * probability 0 adding 0.  top_tokens, top_logprobs [rows][n_top]: the first
- * n_top (at most 32) of that order, past V -1 and -inf.  A row that holds a
- * NaN or +inf, or nothing above -inf, has NaN for every log probability
- * within V and for its entropy.  NULL outputs are left out (top_tokens and
- * top_logprobs go together); no output may overlap another argument.  ws: cgx_token_logprobs_ws bytes of device memory
+ * than 2^23 rows, V at most 2^30), device pointers throughout.  For the given
+ * token of each row (tokens [rows], NULL: none): logprob = x[tok] - log sum
+ * exp(x) and rank, the number of tokens before it in the order (value
+ * descending, index ascending; NaN last); a token outside [0, V) has -inf and
+ * rank V.  entropy: -sum p log p, a token of probability 0 adding 0.
+ * top_tokens, top_logprobs [rows][n_top]: the first n_top (at most 32) of that
+ * order, past V -1 and -inf.  A row that holds a NaN or +inf, or nothing above
+ * -inf, has NaN for every log probability within V and for its entropy.  NULL
+ * outputs are left out (top_tokens and top_logprobs go together); no output may
+ * overlap another argument.  ws: cgx_token_logprobs_ws bytes of device memory
  * (16-byte aligned), as for cgx_attention_paged_dev: enough for every call of
  * at most these rows, V and n_top. */
 size_t cgx_token_logprobs_ws(int rows, int V, int n_top);
