@@ -31,6 +31,12 @@ static int check_shape(const char* who, int layers, int pages, int page, int hea
                       who, layers, pages, page, heads, D, gs);
         return -1;
     }
+    /* byte offsets in 64 bits: a position's head has D / 2 bytes of codes and up to 2 D of scales */
+    if ((double)pages * page * heads * layers * (2.0 * D) > (double)(1LL << 60)) {
+        cgx_set_error("%s: %d layers of %d pages of %d positions, %d heads of %d are too large",
+                      who, layers, pages, page, heads, D);
+        return -1;
+    }
     return 0;
 }
 

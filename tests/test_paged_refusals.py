@@ -102,3 +102,14 @@ def test_logprobs_of_overlapping_memory(lib):
     for kw in (dict(lp=x + 1596), dict(rank=tok + 4), dict(ent=lp), dict(top=ent + 4), dict(top_lp=top + 20),
                dict(V=9000, x=P16 + 16384, ws=P16 + 16384), dict(V=9000, x=P16 + 16384, lp=P16 + 4096)):
         assert "overlap" in call(**kw), kw
+
+
+@pytest.mark.parametrize("layers,pages,heads,D", [
+    (1 << 20, (1 << 27) - 1, 1 << 14, 32), (2**31 - 1, (1 << 27) - 1, 2**31 - 1, 256), (1 << 16, 1 << 26, 1 << 18, 64)])
+def test_a_cache_whose_bytes_pass_64_bits(lib, layers, pages, heads, D):
+    """Sizes that would wrap to a small allocation."""
+    assert not lib.cgx_kv_paged_int4_new(layers, pages, 16, heads, D, D)
+    assert "too large" in last_error(lib)
+    lib.cgx_clear_error()
+    c = _cache(num_layers=layers, num_pages=pages, n_heads=heads, head_dim=D, group_size=D)
+    assert "too large" in _error(lib, lib.cgx_kv_paged_gather_dev(C.byref(c), 0, P16, 1, P16 + 4096, P16 + 8192))
