@@ -31,7 +31,7 @@ static int check_shape(const char* who, int layers, int pages, int page, int hea
                       who, layers, pages, page, heads, D, gs);
         return -1;
     }
-    /* byte offsets in 64 bits: a position's head has D / 2 bytes of codes and up to 2 D of scales */
+    /* byte offsets in 64 bits: a position's head has D / 2 bytes of codes, up to 2 D of scales */
     if ((double)pages * page * heads * layers * (2.0 * D) > (double)(1LL << 60)) {
         cgx_set_error("%s: %d layers of %d pages of %d positions, %d heads of %d are too large",
                       who, layers, pages, page, heads, D);
@@ -135,7 +135,8 @@ void cgx_kv_paged_int4_free(cgx_kv_paged_int4* c) {
 }
 
 static int overlap(const int* a, size_t na, const int* b, size_t nb) {
-    return a && b && (uintptr_t)a < (uintptr_t)(b + nb) && (uintptr_t)b < (uintptr_t)(a + na);
+    return a && b && na && nb && (uintptr_t)a < (uintptr_t)(b + nb) &&
+           (uintptr_t)b < (uintptr_t)(a + na);
 }
 
 int cgx_paged_plan_dev(const cgx_paged_step* s, int page_size, int num_pages, int* free_pages,

@@ -440,7 +440,8 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* cache, int layer, const cgx
                             const int* tree_len, float* O, float* lse, void* ws, size_t ws_bytes);
 
 /* Log probabilities of rows of logits x [rows][V] (ld floats apart; fewer
- * than 2^23 rows, V at most 2^30), device pointers throughout.  For the given
+ * than 2^23 rows, V at most 2^30, fewer than 2^24 pieces of 4096 or, of many
+ * rows, 8192 logits in all), device pointers throughout.  For the given
  * token of each row (tokens [rows], NULL: none): logprob = x[tok] - log sum
  * exp(x) and rank, the number of tokens before it in the order (value
  * descending, index ascending; NaN last); a token outside [0, V) has -inf and
