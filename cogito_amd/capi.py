@@ -13,6 +13,10 @@ CG_MAX_DIMS = 8
 CG_MAX_PARENTS = 4
 
 
+# formats of microscaled rows and weights (cg_mi355x.h)
+CGX_MX_FP4, CGX_MX_FP6, CGX_MX_FP32 = 4, 6, 32
+
+
 class CgTensor(C.Structure):
     pass
 
@@ -309,6 +313,17 @@ SIGNATURES: dict[str, tuple] = {
     "cgx_attention_paged_dev": (I, [PPAGED, I, PSTEP, VP, I, VP, VP, VP, VP, VP, SZ]),
     "cgx_token_logprobs_ws": (SZ, [I, I, I]),
     "cgx_token_logprobs_dev": (I, [VP, SZ, I, I, VP, I, VP, VP, VP, VP, VP, VP, SZ]),
+    # microscaled 4-bit weights and the loss over a vocabulary of them
+    "cgx_mx_quantize_dev": (I, [VP, SZ, I, I, I, VP, VP]),
+    "cgx_mx_dequantize_dev": (I, [VP, VP, I, I, I, VP, SZ]),
+    "cgx_mx_weight_new": (VP, [VP, VP, I, I, I]),
+    "cgx_mx_weight_from_tensor": (VP, [PT, I]),
+    "cgx_mx_weight_free": (None, [VP]),
+    "cgx_matmul_mx_ws": (SZ, [VP, I, I]),
+    "cgx_matmul_mx_dev": (I, [VP, SZ, I, VP, I, VP, SZ, VP, SZ]),
+    "cgx_token_loss_mx_ws": (SZ, [VP, I, I, I]),
+    "cgx_token_loss_mx_dev": (I, [VP, SZ, I, VP, I, VP, VP, VP, VP, SZ]),
+    "cgx_token_loss_mx_grad_dev": (I, [VP, SZ, I, VP, I, VP, VP, VP, VP, SZ, VP, SZ]),
     # synthetic decoder and the speculative loop
     "cgx_model_new": (VP, [C.POINTER(CgxModelConfig), C.c_uint64, VP]),
     "cgx_model_free": (None, [VP]),

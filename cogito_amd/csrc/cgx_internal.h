@@ -36,6 +36,16 @@ int cgx_is_capturing(void);
  * device pointer, else copies `bytes` into scratch `slot`. */
 const void* cgx_dev_in(const void* p, size_t bytes, int slot);
 
+/* Memory of a call: blocks read inputs while others write outputs, so that an
+ * output may lie over nothing else.  The first, an output, may be span `place`
+ * (-1: none) where both start alike.  -1 with the error set otherwise. */
+typedef struct {
+    const void* p;
+    size_t n;        /* bytes */
+    int out;
+} cgx_span;
+int cgx_check_spans(const char* who, const cgx_span* s, int n, int place);
+
 /* ------------------------------------------------ quantized-weight registry */
 enum { CGX_LAYOUT_HOST = 0, CGX_LAYOUT_FLAT = 1, CGX_LAYOUT_TILED = 2, CGX_LAYOUT_MFMA = 3 };
 typedef struct {
@@ -289,6 +299,50 @@ size_t cgk_logprobs_need(int rows, int V, int n_top);    /* of this one */
 int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens, int n_top,
                  float* logprob, int* rank, float* entropy, int* top_tokens,
                  float* top_logprobs, void* ws);
+
+/* Microscaled weights (mx.hip, mx_loss.hip); arguments checked by host/mx.c.
+ * A weight is records of 256 outputs and 128 inputs; with a gradient also its
+ * transpose, records of 256 inputs and a chunk of 128 outputs, first[c] ..
+ * first[c + 1] - 1 those of chunk c (list: the chunk of each). */
+struct cgx_mx_weight {
+    int K, N;
+    uint8_t* codes;
+    int chunks128;           /* chunks of 128 outputs */
+    uint8_t* tcodes;         /* NULL: no gradient */
+    int* list;               /* device, [tchunks] */
+    int* first;              /* host, [chunks128 + 1] */
+    int tchunks;
+};
+int cgk_mx_quantize(const float* x, size_t ld, int rows, int cols, int format, uint8_t* codes,
+                    uint8_t* scales);
+int cgk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int cols, int format,
+                      float* y, size_t ld);
+size_t cgk_mx_weight_bytes(int K, int N);
+int cgk_mx_weight(const uint8_t* codes, const uint8_t* scales, int K, int N, uint8_t* w);
+int cgk_mx_weight_of(const float* x, int K, int N, uint8_t* w);
+int cgk_mx_layers(const uint8_t* w, int K, int N, int* layers);
+size_t cgk_mx_transposed_bytes(int K, int chunks);
+int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list, const int* first,
+                      int chunks, uint8_t* out);
+/* records of rows, in blocks of mt tiles of 16 */
+int cgk_mx_tiles(int M);
+size_t cgk_mx_rows_bytes(int M, int K, int act, int mt);
+int cgk_mx_rows(const float* x, size_t ld, int M, int K, int act, int mt, uint8_t* out);
+/* y[m][n] (+)= row_scale[m] * the sum of `splits` parts, 0 in rows whose
+ * target is none of V (targets NULL: none) */
+int cgk_mx_join(const float* part, int splits, size_t stride, int pld, int M, int N, float* y,
+                size_t ld, const float* row_scale, const int* targets, int V, int add);
+size_t cgk_mx_matmul_need(const cgx_mx_weight* w, int M, int act);   /* of this call */
+size_t cgk_mx_matmul_ws(const cgx_mx_weight* w, int M, int act);     /* of any up to M rows */
+int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_weight* w, int act, float* y,
+                  size_t ldy, void* ws);
+size_t cgk_mx_loss_need(const cgx_mx_weight* w, int M, int act, int grad);
+size_t cgk_mx_loss_ws(const cgx_mx_weight* w, int M, int act, int grad);
+int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight* w, int act,
+                const int* targets, float* loss, float* lse, void* ws);
+int cgk_mx_loss_grad(const float* x, size_t ld, int M, const cgx_mx_weight* w, int act,
+                     const int* targets, const float* lse, const float* dloss, float* dx,
+                     size_t ldd, void* ws);
 
 /* Rows of a tree forward (cgx_model_forward_tree): row i sits at cache slot
  * len + i and rotary position len + rel[i]; the last tw cached keys are the

@@ -60,15 +60,7 @@ static int check_cache(const char* who, const cgx_kv_paged_int4* c, int layer) {
     return 0;
 }
 
-/* Memory of a call: blocks read inputs while others write outputs, so that an
- * output may lie over nothing else.  The first, an output, may be span `place`
- * (-1: none) where both start alike. */
-typedef struct {
-    const void* p;
-    size_t n;        /* bytes */
-    int out;
-} span;
-static int check_spans(const char* who, const span* s, int n, int place) {
+int cgx_check_spans(const char* who, const cgx_span* s, int n, int place) {
     for (int i = 0; i < n; i++)
         for (int j = 0; s[i].out && j < n; j++) {
             const uintptr_t a = (uintptr_t)s[i].p, b = (uintptr_t)s[j].p;
@@ -201,14 +193,14 @@ int cgx_kv_paged_append_dev(cgx_kv_paged_int4* c, int layer, const cgx_paged_ste
         return -1;
     }
     const size_t T = (size_t)s->rows, D = (size_t)c->head_dim;
-    const span mem[] = {
+    const cgx_span mem[] = {
         {q_out, T * H * D * 4, 1},
         {qkv, T ? ((T - 1) * ldq + (H + 2 * (size_t)c->n_heads) * D) * 4 : 0, 0},
         {rope, (size_t)(rope ? rope_rows : 0) * D * 4, 0},
         {s->row_slot, T * 4, 0},
         {rope ? s->row_pos : NULL, T * 4, 0}};
     /* one row may be rotated in its place: a thread's values are its own */
-    if (check_spans(who, mem, 5, T == 1 ? 1 : -1)) return -1;
+    if (cgx_check_spans(who, mem, 5, T == 1 ? 1 : -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!s->rows) return 0;
     return cgk_paged_append(c, layer, s, qkv, ldq, H, rope, rope_rows, q_out);
@@ -224,8 +216,8 @@ int cgx_kv_paged_gather_dev(const cgx_kv_paged_int4* c, int layer, const int* sl
         return -1;
     }
     const size_t bytes = (size_t)n * c->n_heads * c->head_dim * 4;
-    const span mem[] = {{k, bytes, 1}, {v, bytes, 1}, {slots, (size_t)n * 4, 0}};
-    if (check_spans(who, mem, 3, -1)) return -1;
+    const cgx_span mem[] = {{k, bytes, 1}, {v, bytes, 1}, {slots, (size_t)n * 4, 0}};
+    if (cgx_check_spans(who, mem, 3, -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!n) return 0;
     return cgk_paged_gather(c, layer, slots, n, k, v);
@@ -286,7 +278,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
         return -1;
     }
     const size_t T = (size_t)s->rows, B = (size_t)s->seqs;
-    const span mem[] = {{O, T * H * c->head_dim * 4, 1},
+    const cgx_span mem[] = {{O, T * H * c->head_dim * 4, 1},
                         {lse, T * H * 4, 1},
                         {ws, need, 1},
                         {Q, T * H * c->head_dim * 4, 0},
@@ -297,7 +289,7 @@ int cgx_attention_paged_dev(const cgx_kv_paged_int4* c, int layer, const cgx_pag
                         {anc, T * 8, 0},
                         {tree_len, B * 4, 0}};
     /* O in the place of Q: a block writes the rows and heads that it has read */
-    if (check_spans(who, mem, 10, 3)) return -1;
+    if (cgx_check_spans(who, mem, 10, 3)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!s->rows) return 0;
     return cgk_paged_attention(c, layer, s, Q, H, anc, tree_len, O, lse, ws);
@@ -336,7 +328,7 @@ int cgx_token_logprobs_dev(const float* x, size_t ld, int rows, int V, const int
         return -1;
     }
     const size_t T = (size_t)rows;
-    const span mem[] = {{logprob, T * 4, 1},
+    const cgx_span mem[] = {{logprob, T * 4, 1},
                         {rank, T * 4, 1},
                         {entropy, T * 4, 1},
                         {top_tokens, T * n_top * 4, 1},
@@ -344,7 +336,7 @@ int cgx_token_logprobs_dev(const float* x, size_t ld, int rows, int V, const int
                         {ws, need, 1},
                         {x, T ? ((T - 1) * ld + V) * 4 : 0, 0},
                         {tokens, T * 4, 0}};
-    if (check_spans(who, mem, 8, -1)) return -1;
+    if (cgx_check_spans(who, mem, 8, -1)) return -1;
     if (cgx_ensure_init()) return -1;
     if (!rows) return 0;
     return cgk_logprobs(x, ld, rows, V, tokens, n_top, logprob, rank, entropy, top_tokens,

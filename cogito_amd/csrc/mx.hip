@@ -1,0 +1,500 @@
+// mx.hip -- microscaled blocks (32 values and a power of two): quantisation and
+// read-back, the records of a 4-bit weight, and the product of rows with it.
+#include "mx.hpp"
+
+#include <algorithm>
+
+namespace {
+
+using namespace mx;
+
+inline hipStream_t stream() { return (hipStream_t)cgx_stream(); }
+
+int launch_check(const char* what) {
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+        cgx_set_error("%s launch failed: %s", what, hipGetErrorString(e));
+        return -1;
+    }
+    return 0;
+}
+
+inline int up(long long a, int b) { return (int)((a + b - 1) / b); }
+
+// ------------------------------------------------- quantise and read back
+// Four lanes a block, eight values each; a wave takes 16 blocks of one row.
+// The 6-bit conversion takes 32 values: a lane's eight go first and their six
+// bytes are kept.
+__device__ __forceinline__ void load8(float* v, const float* x, int k, int cols, bool vec) {
+    if (vec && k + 8 <= cols) {
+        const f4 a = *(const f4*)(x + k), b = *(const f4*)(x + k + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? x[k + i] : 0.0f;
+    }
+}
+
+template <int FMT>
+__global__ __launch_bounds__(256) void k_quantize(const float* __restrict__ x, size_t ld, int rows,
+                                                  int cols, int segs, bool vec,
+                                                  uint8_t* __restrict__ codes,
+                                                  uint8_t* __restrict__ scales) {
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int row = wave / segs, seg = wave - row * segs, blocks = (cols + 31) / 32;
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63, blk = seg * 16 + (lane >> 2), part = lane & 3;
+    float v[8];
+    load8(v, x + (size_t)row * ld, blk * 32 + part * 8, cols, vec);
+    int top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int b = __float_as_int(v[i]) & 0x7fffffff;
+        top = b > top ? b : top;
+    }
+    int o = __shfl_xor(top, 1);
+    top = o > top ? o : top;
+    o = __shfl_xor(top, 2);
+    top = o > top ? o : top;
+    top >>= 23;
+    const int byte = top == 255 ? 255 : top > 3 ? top - 2 : 1;
+    if (blk >= blocks) return;
+    const float s = pow2(byte == 255 ? 127 : byte);
+    const size_t at = (size_t)row * blocks + blk;
+    if (part == 0) scales[at] = (uint8_t)byte;
+    if constexpr (FMT == CGX_MX_FP4) {
+        unsigned r = 0;
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
+        *(unsigned*)(codes + at * 16 + part * 4) = r;
+    } else {
+        f16 a = {}, b = {};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            a[i] = v[2 * i];
+            b[i] = v[2 * i + 1];
+        }
+        const u6 q = to6<kE2M3>(a, b, s);
+        uint16_t* p = (uint16_t*)(codes + at * 24 + part * 6);
+        p[0] = (uint16_t)q[0];
+        p[1] = (uint16_t)(q[0] >> 16);
+        p[2] = (uint16_t)q[1];
+    }
+}
+
+__device__ __forceinline__ float value4(int q) {
+    const int e = (q >> 1) & 3;
+    const float m = e ? __int_as_float(((e + 126) << 23) | (q & 1) << 22) : (q & 1) * 0.5f;
+    return q & 8 ? -m : m;
+}
+__device__ __forceinline__ float value6(int q) {
+    const int e = (q >> 3) & 3;
+    const float m = e ? __int_as_float(((e + 126) << 23) | (q & 7) << 20) : (q & 7) * 0.125f;
+    return q & 32 ? -m : m;
+}
+
+template <int FMT>
+__global__ __launch_bounds__(256) void k_dequantize(const uint8_t* __restrict__ codes,
+                                                    const uint8_t* __restrict__ scales, int rows,
+                                                    int cols, int segs, bool vec,
+                                                    float* __restrict__ y, size_t ld) {
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int row = wave / segs, seg = wave - row * segs, blocks = (cols + 31) / 32;
+    const int lane = threadIdx.x & 63, blk = seg * 16 + (lane >> 2), part = lane & 3;
+    if (row >= rows || blk >= blocks) return;
+    const size_t at = (size_t)row * blocks + blk;
+    const int byte = scales[at], k = blk * 32 + part * 8;
+    float v[8];
+    if constexpr (FMT == CGX_MX_FP4) {
+        const unsigned r = *(const unsigned*)(codes + at * 16 + part * 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = value4((r >> (4 * i)) & 15);
+    } else {
+        const uint16_t* p = (const uint16_t*)(codes + at * 24 + part * 6);
+        const unsigned long long r = p[0] | (unsigned long long)p[1] << 16 | (unsigned long long)p[2] << 32;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = value6((int)(r >> (6 * i)) & 63);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = byte == 255 ? NAN : ldexpf(v[i], byte - 127);
+    float* o = y + (size_t)row * ld + k;
+    if (vec && k + 8 <= cols) {
+        *(f4*)o = f4{v[0], v[1], v[2], v[3]};
+        *(f4*)(o + 4) = f4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (k + i < cols) o[i] = v[i];
+    }
+}
+
+// ------------------------------------------------------ weight records
+// From rows of codes [N][blocks * 16] and scales [N][blocks]: a wave a tile
+// (16 outputs) and chunk.  Outputs past N and blocks past K are 0.
+__global__ __launch_bounds__(256) void k_weight(const uint8_t* __restrict__ codes,
+                                                const uint8_t* __restrict__ scales, int N,
+                                                int blocks, int kc, long long units,
+                                                uint8_t* __restrict__ w) {
+    const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= units) return;
+    const int lane = threadIdx.x & 63, t = (int)(u % 16);
+    const long long rec = u / 16;
+    const int c = (int)(rec % kc), n = (int)(rec / kc) * 256 + t * 16 + (lane & 15);
+    const int blk = c * 4 + (lane >> 4);
+    i4 q = {0, 0, 0, 0};
+    int s = 127;
+    if (n < N && blk < blocks) {
+        const size_t at = (size_t)n * blocks + blk;
+        q = *(const i4*)(codes + at * 16);
+        s = scales[at];
+    }
+    uint8_t* p = w + (size_t)rec * kWRecord;
+    *(i4*)(p + t * 1024 + lane * 16) = q;
+    p[kWTiles * 1024 + t * 64 + lane] = (uint8_t)s;
+}
+
+// From a matrix [K][N], quantised along K: a thread an output and block.
+__global__ __launch_bounds__(256) void k_weight_of(const float* __restrict__ x, int K, int N,
+                                                   int kc, uint8_t* __restrict__ w) {
+    const int n = blockIdx.x * 256 + threadIdx.x, blk = blockIdx.y, c = blk >> 2;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        const int k = blk * 32 + i;
+        v[i] = n < N && k < K ? x[(size_t)k * N + n] : 0.0f;
+    }
+    const Cut<CGX_MX_FP4> q = cut<CGX_MX_FP4>(v);
+    uint8_t* p = w + ((size_t)blockIdx.x * kc + c) * kWRecord;
+    const int t = threadIdx.x >> 4, lane = (blk & 3) * 16 + (threadIdx.x & 15);
+    *(i4*)(p + t * 1024 + lane * 16) = i4{q.q[0][0], q.q[0][1], q.q[0][2], q.q[0][3]};
+    p[kWTiles * 1024 + t * 64 + lane] = (uint8_t)q.byte;
+}
+
+// ------------------------------------------------- transposed records
+// For the gradient the contraction runs along the outputs, so a block is 32
+// outputs of one input.  A weight's value is +-m 2^(s - 127), m in {.5 .. 6}, and s
+// differs from output to output; E3M2 holds 4 m 2^-d for d = 0 .. 5 exactly.
+// With top the block's largest s, layer p takes the outputs with top - s in
+// 6 p .. 6 p + 5, under the scale 2^(top - 6 p - 2 - 127), so that the layers' sum
+// is the weight exactly.  One layer holds nearly every block; a chunk (128
+// outputs) has as many as its worst block needs, each a chunk of the
+// contraction of its own.
+__device__ __forceinline__ int code_at(const uint8_t* w, int kc, int n, int k, int* s) {
+    const uint8_t* p = w + ((size_t)(n >> 8) * kc + (k >> 7)) * kWRecord;
+    const int t = (n >> 4) & 15, lane = ((k >> 5) & 3) * 16 + (n & 15), i = k & 31;
+    *s = p[kWTiles * 1024 + t * 64 + lane];
+    return p[t * 1024 + lane * 16 + (i >> 1)] >> (4 * (i & 1)) & 15;
+}
+
+// Layers of every chunk: a block a chunk and 128 inputs, a thread two blocks' range.
+__global__ __launch_bounds__(256) void k_layers(const uint8_t* __restrict__ w, int N, int K,
+                                                int kc, int* __restrict__ layers) {
+    const int c = blockIdx.x;
+    int need = 1;
+    for (int u = threadIdx.x; u < 512; u += 256) {
+        const int k = blockIdx.y * 128 + (u & 127), n0 = c * 128 + (u >> 7) * 32;
+        if (k >= K) continue;
+        int top = -1, low = 256;
+        for (int i = 0; i < 32 && n0 + i < N; i++) {
+            int s;
+            const int q = code_at(w, kc, n0 + i, k, &s);
+            if (!(q & 7) || s == 255) continue;
+            top = s > top ? s : top;
+            low = s < low ? s : low;
+        }
+        if (top >= 0) need = max(need, (top - low) / 6 + 1);
+    }
+    if (need > 1) atomicMax(&layers[c], need);
+}
+
+// A wave a tile (16 inputs) of a listed chunk and layer.
+__global__ __launch_bounds__(256) void k_transposed(const uint8_t* __restrict__ w, int N, int K,
+                                                    int kc, const int* __restrict__ list,
+                                                    const int* __restrict__ first, int chunks,
+                                                    uint8_t* __restrict__ out) {
+    const int j = blockIdx.x, t = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int c = list[j], layer = j - first[c];
+    const int k = blockIdx.z * 256 + t * 16 + (lane & 15), n0 = c * 128 + (lane >> 4) * 32;
+    int q[32], s[32], top = -1;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        q[i] = 0;
+        s[i] = 0;
+        if (k < K && n0 + i < N) q[i] = code_at(w, kc, n0 + i, k, &s[i]);
+        if (s[i] == 255) nan = true;
+        else if ((q[i] & 7) && s[i] > top) top = s[i];
+    }
+    int byte = top - 6 * layer - 2;
+    byte = byte < 0 ? 0 : byte;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+        v[i] = !nan && (top - s[i]) / 6 == layer ? ldexpf(value4(q[i]), s[i] - byte) : 0.0f;
+    f16 a, b;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        a[i] = v[2 * i];
+        b[i] = v[2 * i + 1];
+    }
+    const u6 r = to6<kE3M2>(a, b, 1.0f);
+    uint8_t* p = out + ((size_t)blockIdx.z * chunks + j) * kTRecord;
+    *(i4*)(p + t * 1536 + lane * 16) = i4{(int)r[0], (int)r[1], (int)r[2], (int)r[3]};
+    *(i2*)(p + t * 1536 + 1024 + lane * 8) = i2{(int)r[4], (int)r[5]};
+    p[kWTiles * 1536 + t * 64 + lane] = (uint8_t)(nan ? 255 : top < 0 ? 127 : byte);
+}
+
+// ------------------------------------------------------- rows' records
+// A wave a tile of 16 rows and a chunk, a lane a block.
+template <int ACT>
+__global__ __launch_bounds__(256) void k_rows(const float* __restrict__ x, size_t ld, int M, int K,
+                                              int kc, int mt, long long units, bool vec,
+                                              uint8_t* __restrict__ out) {
+    const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= units) return;
+    const int lane = threadIdx.x & 63, tile = (int)(u / kc), c = (int)(u - (long long)tile * kc);
+    const int m = tile * 16 + (lane & 15), k = c * 128 + (lane >> 4) * 32;
+    float v[32];
+    const float* p = x + (size_t)m * ld;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (m < M) load8(v + 8 * i, p, k + 8 * i, K, vec);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[8 * i + j] = 0.0f;
+    }
+    using R = Rows<ACT>;
+    const int b = tile / mt, at = tile - b * mt;
+    uint8_t* rec = out + ((size_t)b * kc + c) * (size_t)(mt * (R::tile + 64));
+    put<ACT>(rec + at * R::tile, rec + mt * R::tile + at * 64, lane, cut<ACT>(v));
+}
+
+// Splits of a product in order: y[m][n] (+)= row_scale[m] * sum of part[s][m][n];
+// 0 in a row whose target is none of V.
+__global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int splits,
+                                              size_t stride, int pld, int M, int N,
+                                              float* __restrict__ y, size_t ld, bool vec,
+                                              const float* __restrict__ row_scale,
+                                              const int* __restrict__ targets, int V, int add) {
+    const int q = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y, n = 4 * q;
+    if (n >= N) return;
+    const float* p = part + (size_t)m * pld + n;
+    f4 v = {0, 0, 0, 0};
+    for (int s = 0; s < splits; s += 8) {
+        f4 t[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = *(const f4*)(p + (size_t)min(s + i, splits - 1) * stride);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (s + i < splits) v += t[i];
+    }
+    if (row_scale) v *= row_scale[m];
+    if (targets && (unsigned)targets[m] >= (unsigned)V) v = f4{0, 0, 0, 0};
+    float* o = y + (size_t)m * ld + n;
+    if (vec && n + 3 < N) {
+        if (add) v += *(const f4*)o;
+        *(f4*)o = v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (n + r < N) o[r] = add ? o[r] + v[r] : v[r];
+    }
+}
+
+}  // namespace
+
+// ------------------------------------------------------------ launchers
+extern "C" int cgk_mx_quantize(const float* x, size_t ld, int rows, int cols, int format,
+                               uint8_t* codes, uint8_t* scales) {
+    const int segs = up(cols, 512);
+    const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0;
+    const dim3 grid(up((long long)rows * segs, 4));
+    if (format == CGX_MX_FP4)
+        hipLaunchKernelGGL((k_quantize<CGX_MX_FP4>), grid, dim3(256), 0, stream(), x, ld, rows, cols,
+                           segs, vec, codes, scales);
+    else
+        hipLaunchKernelGGL((k_quantize<CGX_MX_FP6>), grid, dim3(256), 0, stream(), x, ld, rows, cols,
+                           segs, vec, codes, scales);
+    return launch_check("mx quantize");
+}
+
+extern "C" int cgk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                                 int format, float* y, size_t ld) {
+    const int segs = up(cols, 512);
+    const bool vec = ((uintptr_t)y & 15) == 0 && ld % 4 == 0;
+    const dim3 grid(up((long long)rows * segs, 4));
+    if (format == CGX_MX_FP4)
+        hipLaunchKernelGGL((k_dequantize<CGX_MX_FP4>), grid, dim3(256), 0, stream(), codes, scales,
+                           rows, cols, segs, vec, y, ld);
+    else
+        hipLaunchKernelGGL((k_dequantize<CGX_MX_FP6>), grid, dim3(256), 0, stream(), codes, scales,
+                           rows, cols, segs, vec, y, ld);
+    return launch_check("mx dequantize");
+}
+
+extern "C" size_t cgk_mx_weight_bytes(int K, int N) {
+    return (size_t)up(N, 256) * up(K, 128) * kWRecord;
+}
+extern "C" int cgk_mx_weight(const uint8_t* codes, const uint8_t* scales, int K, int N, uint8_t* w) {
+    const int kc = up(K, 128);
+    const long long units = (long long)up(N, 256) * kc * 16;
+    hipLaunchKernelGGL(k_weight, dim3(up(units, 4)), dim3(256), 0, stream(), codes, scales, N,
+                       up(K, 32), kc, units, w);
+    return launch_check("mx weight");
+}
+extern "C" int cgk_mx_weight_of(const float* x, int K, int N, uint8_t* w) {
+    const int kc = up(K, 128);
+    hipLaunchKernelGGL(k_weight_of, dim3(up(N, 256), kc * 4), dim3(256), 0, stream(), x, K, N, kc, w);
+    return launch_check("mx weight of a tensor");
+}
+
+// layers (device, one int a chunk of 128 outputs, 0 before)
+extern "C" int cgk_mx_layers(const uint8_t* w, int K, int N, int* layers) {
+    hipLaunchKernelGGL(k_layers, dim3(up(N, 128), up(K, 128)), dim3(256), 0, stream(), w, N, K,
+                       up(K, 128), layers);
+    return launch_check("mx layers");
+}
+extern "C" size_t cgk_mx_transposed_bytes(int K, int chunks) {
+    return (size_t)up(K, 256) * chunks * kTRecord;
+}
+extern "C" int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list, const int* first,
+                                 int chunks, uint8_t* out) {
+    hipLaunchKernelGGL(k_transposed, dim3(chunks, 4, up(K, 256)), dim3(256), 0, stream(), w, N, K,
+                       up(K, 128), list, first, chunks, out);
+    return launch_check("mx transpose");
+}
+
+// Records of rows, mt tiles each, for the row blocks' whole height.
+extern "C" int cgk_mx_rows(const float* x, size_t ld, int M, int K, int act, int mt, uint8_t* out) {
+    const int kc = up(K, 128);
+    const long long units = (long long)up(M, 16 * mt) * mt * kc;
+    const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0;
+    const dim3 grid(up(units, 4));
+    auto go = [&](auto k) {
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, stream(), x, ld, M, K, kc, mt, units, vec, out);
+    };
+    if (act == CGX_MX_FP4) go(k_rows<CGX_MX_FP4>);
+    else if (act == CGX_MX_FP6) go(k_rows<CGX_MX_FP6>);
+    else go(k_rows<CGX_MX_FP32>);
+    return launch_check("mx rows");
+}
+extern "C" size_t cgk_mx_rows_bytes(int M, int K, int act, int mt) {
+    const size_t rec = act == CGX_MX_FP4 ? rows_record<CGX_MX_FP4>(mt)
+                       : act == CGX_MX_FP6 ? rows_record<CGX_MX_FP6>(mt) : rows_record<CGX_MX_FP32>(mt);
+    return rec * up(M, 16 * mt) * up(K, 128);
+}
+
+extern "C" int cgk_mx_join(const float* part, int splits, size_t stride, int pld, int M, int N,
+                           float* y, size_t ld, const float* row_scale, const int* targets,
+                           int V, int add) {
+    const bool vec = ((uintptr_t)y & 15) == 0 && ld % 4 == 0;
+    hipLaunchKernelGGL(k_join, dim3(up(N, 1024), M), dim3(256), 0, stream(), part, splits, stride,
+                       pld, M, N, y, ld, vec, row_scale, targets, V, add);
+    return launch_check("mx join");
+}
+
+namespace {
+
+constexpr int kSlab = 4096;          // rows a launch: bounds the records' workspace
+
+// How M rows go over a weight: tiles of a row block, blocks, and splits of K
+// where there are fewer than two blocks a CU.
+struct Plan {
+    int mt, mbs, nbs, splits;
+    size_t rows, part;               // bytes
+};
+Plan plan(const cgx_mx_weight* w, int M, int act) {
+    Plan p;
+    p.mt = cgk_mx_tiles(M);
+    p.mbs = up(M, 16 * p.mt);
+    p.nbs = up(w->N, 256);
+    const int kc = up(w->K, 128), blocks = p.mbs * p.nbs;
+    p.splits = std::max(1, std::min(512 / blocks, kc / 4));
+    p.rows = (cgk_mx_rows_bytes(M, w->K, act, p.mt) + 255) & ~(size_t)255;
+    p.part = p.splits > 1 ? (size_t)p.splits * M * ((w->N + 3) & ~3) * 4 : 0;
+    return p;
+}
+
+template <int ACT, int BM, int WM>
+void gemm(const Gemm& g) {
+    hipLaunchKernelGGL((k_gemm<ACT, kE2M1, BM, WM, kStore>), dim3(g.mbs * g.nbs, g.splits),
+                       dim3(128 * WM), 0, stream(), g);
+}
+template <int ACT>
+void gemm(const Gemm& g, int mt) {
+    if (mt == 1) gemm<ACT, 16, 1>(g);
+    else if (mt == 2) gemm<ACT, 32, 1>(g);
+    else if (mt == 4) gemm<ACT, 64, 1>(g);
+    else gemm<ACT, 128, 2>(g);
+}
+
+}  // namespace
+
+// Tiles of a row block: the smallest that holds M rows, at most 128 rows.
+extern "C" int cgk_mx_tiles(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 8; }
+
+extern "C" size_t cgk_mx_matmul_need(const cgx_mx_weight* w, int M, int act) {
+    size_t need = 0;
+    if (M >= kSlab) {
+        const Plan p = plan(w, kSlab, act);
+        need = p.rows + p.part;
+        M %= kSlab;
+    }
+    if (M) {
+        const Plan p = plan(w, M, act);
+        need = std::max(need, p.rows + p.part);
+    }
+    return need;
+}
+// ... of any call of at most M rows
+extern "C" size_t cgk_mx_matmul_ws(const cgx_mx_weight* w, int M, int act) {
+    const int top = std::min(M, kSlab);
+    size_t need = top ? cgk_mx_matmul_need(w, top, act) : 0;
+    for (int m = 16; m < top; m += 16) need = std::max(need, cgk_mx_matmul_need(w, m, act));
+    return need;
+}
+
+extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_weight* w, int act,
+                             float* y, size_t ldy, void* ws) {
+    for (int m0 = 0; m0 < M; m0 += kSlab) {
+        const int m = std::min(kSlab, M - m0);
+        const Plan p = plan(w, m, act);
+        float* ym = y + (size_t)m0 * ldy;
+        uint8_t* rows = (uint8_t*)ws;
+        if (cgk_mx_rows(x + (size_t)m0 * ldx, ldx, m, w->K, act, p.mt, rows)) return -1;
+        const int kc = up(w->K, 128), pld = (w->N + 3) & ~3;
+        Gemm g = {};
+        g.x = rows;
+        g.w = w->codes;
+        g.xk = g.wk = g.j1 = kc;
+        g.mbs = p.mbs;
+        g.nbs = p.nbs;
+        g.splits = p.splits;
+        g.M = m;
+        g.N = w->N;
+        if (p.splits > 1) {
+            g.y = (float*)(rows + p.rows);
+            g.ld = pld;
+            g.stride = (size_t)m * pld;
+            g.vec = 1;
+        } else {
+            g.y = ym;
+            g.ld = ldy;
+            g.vec = ((uintptr_t)ym & 15) == 0 && ldy % 4 == 0;
+        }
+        if (act == CGX_MX_FP4) gemm<CGX_MX_FP4>(g, p.mt);
+        else if (act == CGX_MX_FP6) gemm<CGX_MX_FP6>(g, p.mt);
+        else gemm<CGX_MX_FP32>(g, p.mt);
+        if (launch_check("mx product")) return -1;
+        if (p.splits > 1 &&
+            cgk_mx_join(g.y, p.splits, g.stride, pld, m, w->N, ym, ldy, nullptr, nullptr, 0, 0))
+            return -1;
+    }
+    return 0;
+}

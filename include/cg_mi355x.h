@@ -458,6 +458,77 @@ int cgx_token_logprobs_dev(const float* logits, size_t ld, int rows, int V, cons
                            int n_top, float* logprob, int* rank, float* entropy,
                            int* top_tokens, float* top_logprobs, void* ws, size_t ws_bytes);
 
+/* ------------------------------- microscaled 4-bit weights and the loss */
+/* Microscaled blocks (no counterpart in the reference): 32 neighbouring values
+ * of a row share a power of two, 2^(byte - 127); a value is 4 bits
+ * (CGX_MX_FP4: sign, 2 exponent bits, 1 of mantissa; 0 to 6) or 6
+ * (CGX_MX_FP6: sign, 2 exponent bits, 3 of mantissa; 0 to 7.5).  Codes of a
+ * block are 16 or 24 bytes, the first value in the lowest bits; a row has
+ * ceil(cols / 32) blocks, the last filled up with 0.  The matrix cores multiply
+ * such blocks as they are. */
+enum { CGX_MX_FP4 = 4, CGX_MX_FP6 = 6, CGX_MX_FP32 = 32 };
+
+/* Rows x [rows][cols] (ld floats apart) to codes [rows][blocks][16 or 24]
+ * (16-byte aligned) and scale bytes [rows][blocks].  byte = floor(log2 of the
+ * block's largest magnitude) + 125, at least 1; values are rounded to the
+ * nearest, ties to even, and saturate.  A block that holds a NaN or an infinity
+ * has the byte 255 and reads as NaN.  dequantize reads any byte (0: 2^-127).
+ * Device pointers; rows times ceil(cols / 512) below 2^26; no output may
+ * overlap another argument. */
+int cgx_mx_quantize_dev(const float* x, size_t ld, int rows, int cols, int format,
+                        uint8_t* codes, uint8_t* scales);
+int cgx_mx_dequantize_dev(const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                          int format, float* y, size_t ld);
+
+/* A 4-bit weight W [K][N] (y = x W) laid out in HBM for the products below.
+ * cgx_mx_weight_new takes it as N rows of K inputs: codes [N][ceil(K / 32)][16]
+ * and scales [N][ceil(K / 32)] as cgx_mx_quantize_dev writes them, host or
+ * device; cgx_mx_weight_from_tensor quantises W, [K, N] as in cg_quantize_int4,
+ * host or device, in blocks along K.  grad: 1 for a weight that
+ * cgx_token_loss_mx_grad_dev takes, which keeps a transposed copy as well
+ * (25/32 bytes a value).  K at most 2^20, N at most 2^24, K N at most 2^36.
+ * NULL on an error. */
+typedef struct cgx_mx_weight cgx_mx_weight;
+cgx_mx_weight* cgx_mx_weight_new(const uint8_t* codes, const uint8_t* scales, int K, int N,
+                                 int grad);
+cgx_mx_weight* cgx_mx_weight_from_tensor(cg_tensor* W, int grad);
+void cgx_mx_weight_free(cgx_mx_weight* w);
+
+/* y [M][N] = x' W, x [M][K] rows of floats (ldx and ldy apart).  act says what
+ * x' is: CGX_MX_FP32 x itself (each value held to 2^-23 of the largest of its
+ * block of 32, and to 2^-130), CGX_MX_FP4 or CGX_MX_FP6 x quantised as
+ * cgx_mx_quantize_dev does.  Sums are held in fp32.  A row with a NaN or an
+ * infinity gets NaN, as does every row's output of a weight block of byte 255.
+ * Device pointers; M below 2^23; no output or workspace may overlap another
+ * argument.  ws: cgx_matmul_mx_ws bytes of device memory (16-byte aligned), for
+ * this call alone while it runs; the size is enough for every call of at most
+ * M rows with this weight and act.  Nothing is allocated: the call may be
+ * captured into a graph. */
+size_t cgx_matmul_mx_ws(const cgx_mx_weight* w, int M, int act);
+int cgx_matmul_mx_dev(const float* x, size_t ldx, int M, const cgx_mx_weight* w, int act,
+                      float* y, size_t ldy, void* ws, size_t ws_bytes);
+
+/* Softmax cross entropy over the vocabulary of an lm_head W [K][V], from hidden
+ * rows h [rows][K] (ldh floats apart), without storing a logit: with
+ * z = h' W (h' as in cgx_matmul_mx_dev), lse[m] = log sum exp z[m] and
+ * loss[m] = lse[m] - z[m][targets[m]], 0 for a target outside [0, V) (an
+ * ignored row).  loss or lse may be NULL.  A row with a logit that is NaN or
+ * +inf, or with none above -inf, has NaN (an lse of -inf in the last case).
+ * The gradient: dh[m] (ldd apart) = dloss[m] (softmax(z[m]) - e_target) W^T,
+ * with softmax(z) = exp(z - lse) for the lse that the first call wrote, dloss
+ * [rows] the gradient of each row's loss (NULL: 1), and 0 for an ignored row;
+ * a quantised h' passes its gradient on to h.  dh is written, not added to.
+ * ws: cgx_token_loss_mx_ws bytes (grad: 1 for the gradient, whose size is
+ * enough for both calls), as in cgx_matmul_mx_dev, which says the rest. */
+size_t cgx_token_loss_mx_ws(const cgx_mx_weight* w, int rows, int act, int grad);
+int cgx_token_loss_mx_dev(const float* h, size_t ldh, int rows, const cgx_mx_weight* w, int act,
+                          const int* targets, float* loss, float* lse, void* ws,
+                          size_t ws_bytes);
+int cgx_token_loss_mx_grad_dev(const float* h, size_t ldh, int rows, const cgx_mx_weight* w,
+                               int act, const int* targets, const float* lse,
+                               const float* dloss, float* dh, size_t ldd, void* ws,
+                               size_t ws_bytes);
+
 /* ------------------------------------------------- synthetic decoder */
 /* Decoder-only transformer with INT4 weights resident in HBM, the model the
  * verify stack runs (reference src/layers/transformer.c:26-149 block order,
