@@ -25,20 +25,6 @@ inline int up(long long a, int b) { return (int)((a + b - 1) / b); }
 // Four lanes a block, eight values each; a wave takes 16 blocks of one row.
 // The 6-bit conversion takes 32 values: a lane's eight go first and their six
 // bytes are kept.
-__device__ __forceinline__ void load8(float* v, const float* x, int k, int cols, bool vec) {
-    if (vec && k + 8 <= cols) {
-        const f4 a = *(const f4*)(x + k), b = *(const f4*)(x + k + 4);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? x[k + i] : 0.0f;
-    }
-}
-
 template <int FMT>
 __global__ __launch_bounds__(256) void k_quantize(const float* __restrict__ x, size_t ld, int rows,
                                                   int cols, int segs, bool vec,
@@ -147,15 +133,27 @@ __global__ __launch_bounds__(256) void k_weight(const uint8_t* __restrict__ code
     const long long rec = u / 16;
     const int c = (int)(rec % kc), n = (int)(rec / kc) * 256 + t * 16 + (lane & 15);
     const int blk = c * 4 + (lane >> 4);
-    i4 q = {0, 0, 0, 0};
+    i4 q = {0, 0, 0, 0}, o;
     int s = 127;
     if (n < N && blk < blocks) {
         const size_t at = (size_t)n * blocks + blk;
         q = *(const i4*)(codes + at * 16);
         s = scales[at];
     }
+    // value i to position 2 i, value 16 + i to 2 i + 1
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned v = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int k = 4 * i + j;                          // values k and 16 + k
+            v |= ((unsigned)q[k / 8] >> (4 * (k % 8)) & 15) << (8 * j);
+            v |= ((unsigned)q[2 + k / 8] >> (4 * (k % 8)) & 15) << (8 * j + 4);
+        }
+        o[i] = (int)v;
+    }
     uint8_t* p = w + (size_t)rec * kWRecord;
-    *(i4*)(p + t * 1024 + lane * 16) = q;
+    *(i4*)(p + t * 1024 + lane * 16) = o;
     p[kWTiles * 1024 + t * 64 + lane] = (uint8_t)s;
 }
 
@@ -163,17 +161,15 @@ __global__ __launch_bounds__(256) void k_weight(const uint8_t* __restrict__ code
 __global__ __launch_bounds__(256) void k_weight_of(const float* __restrict__ x, int K, int N,
                                                    int kc, uint8_t* __restrict__ w) {
     const int n = blockIdx.x * 256 + threadIdx.x, blk = blockIdx.y, c = blk >> 2;
-    float v[32];
+    Block v;
 #pragma unroll
     for (int i = 0; i < 32; i++) {
         const int k = blk * 32 + i;
-        v[i] = n < N && k < K ? x[(size_t)k * N + n] : 0.0f;
+        set(v, i, n < N && k < K ? x[(size_t)k * N + n] : 0.0f);
     }
-    const Cut<CGX_MX_FP4> q = cut<CGX_MX_FP4>(v);
     uint8_t* p = w + ((size_t)blockIdx.x * kc + c) * kWRecord;
     const int t = threadIdx.x >> 4, lane = (blk & 3) * 16 + (threadIdx.x & 15);
-    *(i4*)(p + t * 1024 + lane * 16) = i4{q.q[0][0], q.q[0][1], q.q[0][2], q.q[0][3]};
-    p[kWTiles * 1024 + t * 64 + lane] = (uint8_t)q.byte;
+    put<CGX_MX_FP4>(p + t * 1024, p + kWTiles * 1024 + t * 64, lane, v);
 }
 
 // ------------------------------------------------- transposed records
@@ -189,7 +185,7 @@ __device__ __forceinline__ int code_at(const uint8_t* w, int kc, int n, int k, i
     const uint8_t* p = w + ((size_t)(n >> 8) * kc + (k >> 7)) * kWRecord;
     const int t = (n >> 4) & 15, lane = ((k >> 5) & 3) * 16 + (n & 15), i = k & 31;
     *s = p[kWTiles * 1024 + t * 64 + lane];
-    return p[t * 1024 + lane * 16 + (i >> 1)] >> (4 * (i & 1)) & 15;
+    return p[t * 1024 + lane * 16 + (i & 15)] >> (4 * (i >> 4)) & 15;
 }
 
 // Layers of every chunk: a block a chunk and 128 inputs, a thread two blocks' range.
@@ -237,13 +233,10 @@ __global__ __launch_bounds__(256) void k_transposed(const uint8_t* __restrict__ 
 #pragma unroll
     for (int i = 0; i < 32; i++)
         v[i] = !nan && (top - s[i]) / 6 == layer ? ldexpf(value4(q[i]), s[i] - byte) : 0.0f;
-    f16 a, b;
+    Block x;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        a[i] = v[2 * i];
-        b[i] = v[2 * i + 1];
-    }
-    const u6 r = to6<kE3M2>(a, b, 1.0f);
+    for (int i = 0; i < 32; i++) set(x, i, v[i]);
+    const u6 r = to6<kE3M2>(x.a, x.b, 1.0f);
     uint8_t* p = out + ((size_t)blockIdx.z * chunks + j) * kTRecord;
     *(i4*)(p + t * 1536 + lane * 16) = i4{(int)r[0], (int)r[1], (int)r[2], (int)r[3]};
     *(i2*)(p + t * 1536 + 1024 + lane * 8) = i2{(int)r[4], (int)r[5]};
@@ -259,20 +252,14 @@ __global__ __launch_bounds__(256) void k_rows(const float* __restrict__ x, size_
     const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (u >= units) return;
     const int lane = threadIdx.x & 63, tile = (int)(u / kc), c = (int)(u - (long long)tile * kc);
-    const int m = tile * 16 + (lane & 15), k = c * 128 + (lane >> 4) * 32;
-    float v[32];
-    const float* p = x + (size_t)m * ld;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (m < M) load8(v + 8 * i, p, k + 8 * i, K, vec);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[8 * i + j] = 0.0f;
-    }
+    // rows past the last repeat it: nothing of theirs is stored
+    const int m = min(tile * 16 + (lane & 15), M - 1);
+    Block v;
+    load_block(v, x + (size_t)m * ld, c * 128 + (lane >> 4) * 32, K, vec && c * 128 + 128 <= K);
     using R = Rows<ACT>;
     const int b = tile / mt, at = tile - b * mt;
-    uint8_t* rec = out + ((size_t)b * kc + c) * (size_t)(mt * (R::tile + 64));
-    put<ACT>(rec + at * R::tile, rec + mt * R::tile + at * 64, lane, cut<ACT>(v));
+    uint8_t* rec = out + ((size_t)b * kc + c) * (size_t)rows_record<ACT>(mt);
+    put<ACT>(rec + at * R::tile, rec + mt * R::tile + at * 64, lane, v);
 }
 
 // Splits of a product in order: y[m][n] (+)= row_scale[m] * sum of part[s][m][n];
@@ -410,8 +397,9 @@ struct Plan {
     size_t rows, part;               // bytes
 };
 Plan plan(const cgx_mx_weight* w, int M, int act) {
-    Plan p;
-    p.mt = cgk_mx_tiles(M);
+    Plan p = {};
+    if (M <= 16) return p;           // k_gemv
+    p.mt = cgk_mx_tiles(M, w->N, act);
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
     const int kc = up(w->K, 128), blocks = p.mbs * p.nbs;
@@ -421,23 +409,30 @@ Plan plan(const cgx_mx_weight* w, int M, int act) {
     return p;
 }
 
-template <int ACT, int BM, int WM>
-void gemm(const Gemm& g) {
-    hipLaunchKernelGGL((k_gemm<ACT, kE2M1, BM, WM, kStore>), dim3(g.mbs * g.nbs, g.splits),
-                       dim3(128 * WM), 0, stream(), g);
-}
 template <int ACT>
 void gemm(const Gemm& g, int mt) {
-    if (mt == 1) gemm<ACT, 16, 1>(g);
-    else if (mt == 2) gemm<ACT, 32, 1>(g);
-    else if (mt == 4) gemm<ACT, 64, 1>(g);
-    else gemm<ACT, 128, 2>(g);
+    const dim3 grid(g.mbs * g.nbs, g.splits);
+    if (mt == 2) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 2, 2, kStore>), grid, dim3(256), 0, stream(), g);
+    else if (mt == 4) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 4, 2, kStore>), grid, dim3(256), 0, stream(), g);
+    else hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 8, 2, kStore>), grid, dim3(256), 0, stream(), g);
+}
+template <int ACT>
+void gemv(const Gemv& g) {
+    gemv_launch<ACT, kStore>(g, stream());
 }
 
 }  // namespace
 
-// Tiles of a row block: the smallest that holds M rows, at most 128 rows.
-extern "C" int cgk_mx_tiles(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 8; }
+// Tiles of a row block: 128 rows unless 64 leave a tenth fewer rows empty (fp32
+// rows through 4096 x 32000: 1024 rows 304 us, with 64-row blocks 338; 301 rows
+// through 4096 x 128256: 447 us, 412), half where that leaves a CU without two blocks
+// (61 rows through 768 x 50257: 13.6 us with 32 rows, 15.4 with 64).
+extern "C" int cgk_mx_tiles(int M, int N, int act) {
+    (void)act;
+    int mt = 10 * up(M, 128) * 128 <= 11 * up(M, 64) * 64 ? 8 : 4;
+    while (mt > 2 && (long long)up(M, 16 * mt) * up(N, 256) < 512) mt /= 2;
+    return mt;
+}
 
 extern "C" size_t cgk_mx_matmul_need(const cgx_mx_weight* w, int M, int act) {
     size_t need = 0;
@@ -465,9 +460,30 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
     for (int m0 = 0; m0 < M; m0 += kSlab) {
         const int m = std::min(kSlab, M - m0);
         const Plan p = plan(w, m, act);
+        const float* xm = x + (size_t)m0 * ldx;
         float* ym = y + (size_t)m0 * ldy;
+        if (m <= 16) {
+            Gemv g = {};
+            g.x = xm;
+            g.ldx = ldx;
+            g.vecx = ((uintptr_t)xm & 15) == 0 && ldx % 4 == 0;
+            g.w = w->codes;
+            g.M = m;
+            g.K = w->K;
+            g.N = w->N;
+            g.kc = up(w->K, 128);
+            g.y = ym;
+            g.ld = ldy;
+            g.vec = ((uintptr_t)ym & 15) == 0 && ldy % 4 == 0;
+            g.tiles = up(w->N, 16);
+            if (act == CGX_MX_FP4) gemv<CGX_MX_FP4>(g);
+            else if (act == CGX_MX_FP6) gemv<CGX_MX_FP6>(g);
+            else gemv<CGX_MX_FP32>(g);
+            if (launch_check("mx product of few rows")) return -1;
+            continue;
+        }
         uint8_t* rows = (uint8_t*)ws;
-        if (cgk_mx_rows(x + (size_t)m0 * ldx, ldx, m, w->K, act, p.mt, rows)) return -1;
+        if (cgk_mx_rows(xm, ldx, m, w->K, act, p.mt, rows)) return -1;
         const int kc = up(w->K, 128), pld = (w->N + 3) & ~3;
         Gemm g = {};
         g.x = rows;

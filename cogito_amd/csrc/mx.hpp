@@ -46,9 +46,10 @@ struct Rows {
     // smallest scale byte: the last term's power of two stays above 2^-127
     static constexpr int low = ACT == CGX_MX_FP32 ? 19 : 1;
 };
-// bytes of a chunk's record: tiles' codes, then 64 scale bytes a tile
+// bytes of a chunk's record: tiles' codes, then 64 scale bytes a tile, up to
+// whole KiB (what a wave copies to LDS at a time)
 template <int ACT>
-constexpr int rows_record(int tiles) { return tiles * (Rows<ACT>::tile + 64); }
+constexpr int rows_record(int tiles) { return (tiles * (Rows<ACT>::tile + 64) + 1023) & ~1023; }
 constexpr int kWTiles = 16;                        // 256 outputs a record
 constexpr int kWRecord = kWTiles * (1024 + 64);    // the weight
 constexpr int kTRecord = kWTiles * (1536 + 64);    // its transpose, E3M2
@@ -58,21 +59,32 @@ constexpr int term_shift(int t) { return t ? 5 * t - 2 : 0; }
 
 __device__ __forceinline__ float pow2(int byte) { return __int_as_float(byte << 23); }
 
-// 32 values of a block: scale byte (floor(log2 max) - 2, at least low; 255 for
-// a NaN or an infinity) and codes.
-__device__ __forceinline__ int block_byte(const float* v, int low) {
+// 32 values of a block, the first 16 in a.  The 6-bit conversion takes two
+// vectors of 16 and interleaves them, so a block's codes hold value i at
+// position 2 i and value 16 + i at 2 i + 1, in every record here, rows' and
+// weights' alike: the order within a block does not change a product.
+struct Block {
+    f16 a, b;
+};
+__device__ __forceinline__ void set(Block& x, int i, float v) {
+    if (i < 16) x.a[i] = v;
+    else x.b[i - 16] = v;
+}
+
+// Scale byte: floor(log2 max) - 2, at least low; 255 for a NaN or an infinity.
+__device__ __forceinline__ int block_byte(const Block& x, int low) {
     int top = 0;
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-        const int b = __float_as_int(v[i]) & 0x7fffffff;
-        top = b > top ? b : top;
+    for (int i = 0; i < 16; i++) {
+        const int p = __float_as_int(x.a[i]) & 0x7fffffff, q = __float_as_int(x.b[i]) & 0x7fffffff;
+        top = max(top, max(p, q));
     }
     top >>= 23;
     return top == 255 ? 255 : top - 2 > low ? top - 2 : low;
 }
 
-// 32 values (even ones in a, odd ones in b) over `scale` to 6 bits, to nearest
-// even and saturating.  The instruction writes its result while it still reads
+// 32 values over `scale` to 6 bits, to nearest even and saturating, b's behind
+// a's.  The instruction writes its result while it still reads
 // its operands, which the compiler does not know: the empty statement keeps
 // them in registers of their own until it is done.
 template <int FMT>
@@ -89,72 +101,91 @@ __device__ __forceinline__ f32 from6(u6& q, float scale) {
     return w;
 }
 
-// One 6-bit term of v (rounded to nearest even at 2^e, saturating); v keeps
-// the rest.
-template <bool LAST>
-__device__ __forceinline__ u6 cut6(float* v, float scale) {
-    f16 a, b;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        a[i] = v[2 * i];
-        b[i] = v[2 * i + 1];
-    }
-    u6 q = to6<kE2M3>(a, b, scale);
-    if (!LAST) {
-        const f32 w = from6(q, scale);
-#pragma unroll
-        for (int i = 0; i < 32; i++) v[i] -= w[i];   // exact
-    }
-    return q;
-}
-__device__ __forceinline__ i4 cut4(const float* v, float scale) {
+__device__ __forceinline__ i4 to4(const Block& x, float scale) {
     i4 q;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         unsigned r = 0;
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[8 * w], v[8 * w + 1], scale, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[8 * w + 2], v[8 * w + 3], scale, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[8 * w + 4], v[8 * w + 5], scale, 2);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[8 * w + 6], v[8 * w + 7], scale, 3);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.a[4 * w], x.b[4 * w], scale, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.a[4 * w + 1], x.b[4 * w + 1], scale, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.a[4 * w + 2], x.b[4 * w + 2], scale, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.a[4 * w + 3], x.b[4 * w + 3], scale, 3);
         q[w] = (int)r;
     }
     return q;
 }
 
-// A lane's block as operands: q[t] for term t.
-template <int ACT>
-struct Cut {
-    i8 q[Rows<ACT>::terms];
-    int byte;
-};
-template <int ACT>
-__device__ __forceinline__ Cut<ACT> cut(float* v) {
-    Cut<ACT> c;
-    c.byte = block_byte(v, Rows<ACT>::low);
-    const float s = pow2(c.byte == 255 ? 127 : c.byte);
+// A lane's block as operands: f(t, codes) for each term t, the largest first;
+// returns the scale byte.  x is left with what the last term rounded away.
+template <int ACT, class F>
+__device__ __forceinline__ int cut(Block& x, F f) {
+    const int byte = block_byte(x, Rows<ACT>::low), e = byte == 255 ? 127 : byte;
     if constexpr (ACT == CGX_MX_FP4) {
-        const i4 q = cut4(v, s);
-        c.q[0] = i8{q[0], q[1], q[2], q[3], 0, 0, 0, 0};
+        const i4 q = to4(x, pow2(e));
+        f(0, i8{q[0], q[1], q[2], q[3], 0, 0, 0, 0});
     } else {
 #pragma unroll
         for (int t = 0; t < Rows<ACT>::terms; t++) {
-            const float st = pow2((c.byte == 255 ? 127 : c.byte) - term_shift(t));
-            const u6 q = t + 1 < Rows<ACT>::terms ? cut6<false>(v, st) : cut6<true>(v, st);
-            c.q[t] = i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)q[4], (int)q[5], 0, 0};
+            const float scale = pow2(e - term_shift(t));
+            u6 q = to6<kE2M3>(x.a, x.b, scale);
+            if (t + 1 < Rows<ACT>::terms) {
+                const f32 w = from6(q, scale);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {       // exact
+                    x.a[i] -= w[2 * i];
+                    x.b[i] -= w[2 * i + 1];
+                }
+            }
+            f(t, i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)q[4], (int)q[5], 0, 0});
         }
     }
-    return c;
+    return byte;
 }
 // ... into the record's tile (codes at `tile`, scales at `sc`)
 template <int ACT>
-__device__ __forceinline__ void put(uint8_t* tile, uint8_t* sc, int lane, const Cut<ACT>& c) {
-#pragma unroll
-    for (int t = 0; t < Rows<ACT>::terms; t++) {
+__device__ __forceinline__ void put(uint8_t* tile, uint8_t* sc, int lane, Block& x) {
+    sc[lane] = (uint8_t)cut<ACT>(x, [&](int t, i8 q) {
         uint8_t* p = tile + t * Rows<ACT>::term;
-        *(i4*)(p + lane * 16) = i4{c.q[t][0], c.q[t][1], c.q[t][2], c.q[t][3]};
-        if constexpr (ACT != CGX_MX_FP4) *(i2*)(p + 1024 + lane * 8) = i2{c.q[t][4], c.q[t][5]};
+        *(i4*)(p + lane * 16) = i4{q[0], q[1], q[2], q[3]};
+        if constexpr (ACT != CGX_MX_FP4) *(i2*)(p + 1024 + lane * 8) = i2{q[4], q[5]};
+    });
+}
+
+// Eight values of a row from k on, 0 past its end.
+__device__ __forceinline__ void load8(float* v, const float* x, int k, int cols, bool vec) {
+    if (vec && k + 8 <= cols) {
+        const f4 a = *(const f4*)(x + k), b = *(const f4*)(x + k + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? x[k + i] : 0.0f;
     }
-    sc[lane] = (uint8_t)c.byte;
+}
+// The block from value k of a row on, 0 past the row's end.  vec: every lane's
+// block lies within 16-byte aligned rows; the loads go to where the conversion
+// reads, so that they stay in flight until then.
+__device__ __forceinline__ void load_block(Block& b, const float* x, int k, int cols, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f4 v = *(const f4*)(x + k + 4 * i), w = *(const f4*)(x + k + 16 + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                b.a[4 * i + j] = v[j];
+                b.b[4 * i + j] = w[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const float v = x[min(k + i, cols - 1)];
+            set(b, i, k + i < cols ? v : 0.0f);
+        }
+    }
 }
 
 template <int FMT>
@@ -173,12 +204,13 @@ __device__ __forceinline__ f4 mfma(i8 a, i8 b, f4 c, int sa, int sb) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, FA, FB, 0, sa, 0, sb);
 }
 
-// One KiB (or its first n bytes) straight into LDS, 16 bytes a lane.
-__device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l, int lane, int n) {
-    if (lane * 16 < n)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(g + lane * 16),
-            (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
+
+// One KiB straight into LDS, 16 bytes a lane.
+__device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l, int lane) {
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(g + (unsigned)(lane * 16)),
+        (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
 // What a product's epilogue needs.
@@ -207,6 +239,7 @@ struct Gemm {
     const float* lse;
     uint8_t* p;
     int pk, pmt, pmbs;     // chunks of p, tiles of a record, row blocks
+    int precord;
 };
 
 enum { kStore = 0, kGrad = 1, kStats = 2, kProbs = 3 };
@@ -215,11 +248,11 @@ enum { kStore = 0, kGrad = 1, kStats = 2, kProbs = 3 };
 // holds outputs 16 n + 4 g + r of its row (acc[n][r]); block b of 32 outputs is
 // tiles 2 b and 2 b + 1.  Two swaps of lane halves and quarters transpose
 // groups and blocks, after which group b holds its block's 32 values in order.
-__device__ __forceinline__ void probs(float* v, const f4* acc, int col0, int N, int t, bool live,
+__device__ __forceinline__ void probs(Block& v, const f4* acc, int col0, int N, int t, bool live,
                                       float lse) {
     unsigned q[2][4][4];                                        // [half][r][block]
 #pragma unroll
-    for (int n = 0; n < 8; n++)
+    for (int n = 0; n < 8; n++) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int c = col0 + 16 * n + r;
@@ -227,6 +260,8 @@ __device__ __forceinline__ void probs(float* v, const f4* acc, int col0, int N, 
             if (live && c == t) p = expm1f(acc[n][r] - lse);
             q[n & 1][r][n >> 1] = __float_as_uint(p);
         }
+        __builtin_amdgcn_sched_barrier(0);                    // few registers beside the sums
+    }
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -245,25 +280,57 @@ __device__ __forceinline__ void probs(float* v, const f4* acc, int col0, int N, 
                 b[k + 1] = s[1];
             }
 #pragma unroll
-            for (int g = 0; g < 4; g++) v[16 * h + 4 * g + r] = __uint_as_float(b[g]);
+            for (int g = 0; g < 4; g++) set(v, 16 * h + 4 * g + r, __uint_as_float(b[g]));
         }
 }
 
-// Product of BM rows and 256 outputs a block: the weight's tile is the first
-// operand, so that a lane holds four neighbouring outputs of one row.  A wave
-// has BM / WM rows and 128 outputs.  Records of a chunk go into LDS without
-// passing registers; two blocks a CU overlap one's loads with the other's
-// matrix instructions.
-template <int ACT, int WFMT, int BM, int WM, int EPI>
-__global__ __launch_bounds__(128 * WM, WFMT == kE2M1 ? 2 : 1) void k_gemm(const Gemm a) {
-    constexpr int MT = BM / 16, TM = MT / WM, TN = 8, NW = 2 * WM;
+// A row's maximum and sum over a lane's logits v[n][r] (outputs col + 16 n + r)
+// and those of the lanes that share the row, and its target's logit.
+template <int TN>
+__device__ __forceinline__ float2 stats(f4* v, int col, int N, int t, float* zt) {
+    float top = -INFINITY, mine = 0.0f;
+    if ((unsigned)t >= (unsigned)N) t = -1;
+    const int at = t - col;                                   // 16 n + r where the target is here
+#pragma unroll
+    for (int n = 0; n < TN; n++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            v[n][r] = 16 * n + r < N - col ? v[n][r] : -INFINITY;
+            mine = at == 16 * n + r ? v[n][r] : mine;
+            top = fmaxf(top, v[n][r]);
+        }
+        __builtin_amdgcn_sched_barrier(0);                    // few registers beside the logits
+    }
+    if (t >= 0 && at >= 0 && at < 16 * TN && (at & 15) < 4) *zt = mine;
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // nothing above -inf: the sum is 0, or NaN where a logit is
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < TN; n++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum += expf(v[n][r] - ref);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    return make_float2(top, sum);
+}
+
+// Product of 16 MT rows and 256 outputs a block of WM x 2 waves.  The weight's
+// tile is the first operand, so that a lane holds four neighbouring outputs of
+// one row.  A step takes a chunk; its records go into LDS without passing
+// registers.
+template <int ACT, int WFMT, int MT, int WM, int EPI>
+__global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 3 : 4) void k_gemm(const Gemm a) {
+    constexpr int WN = 2, TM = MT / WM, TN = kWTiles / WN, NW = WM * WN;
     using R = Rows<ACT>;
     constexpr int XR = rows_record<ACT>(MT), WT = WFMT == kE2M1 ? 1024 : 1536;
-    constexpr int WR = kWTiles * (WT + 64), XU = (XR + 1023) / 1024, WU = (WR + 1023) / 1024;
+    constexpr int WR = WFMT == kE2M1 ? kWRecord : kTRecord, XU = XR / 1024, U = XU + WR / 1024;
     __shared__ __attribute__((aligned(16))) uint8_t lds[XR + WR];
-    uint8_t *const lx = lds, *const lw = lds + XR;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // each XCD (block b runs on XCD b % 8) takes a run of outputs with all their rows
     const int nblk = a.mbs * a.nbs, per = nblk / 8, b = blockIdx.x;
     const int sb = b < per * 8 ? (b % 8) * per + b / 8 : b;
@@ -279,19 +346,21 @@ __global__ __launch_bounds__(128 * WM, WFMT == kE2M1 ? 2 : 1) void k_gemm(const 
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f4{0, 0, 0, 0};
 
+    int xj = a.list ? a.list[j0] - a.list0 : j0;
     for (int j = j0; j < j1; j++) {
-        const uint8_t* gx = xb + (size_t)(a.list ? a.list[j] - a.list0 : j) * XR;
+        const uint8_t* gx = xb + (size_t)xj * XR;
         const uint8_t* gw = wb + (size_t)j * WR;
 #pragma unroll
-        for (int u = 0; u < XU; u += NW)
-            if (u + wave < XU)
-                to_lds(gx + (u + wave) * 1024, lx + (u + wave) * 1024, lane, XR - (u + wave) * 1024);
-#pragma unroll
-        for (int u = 0; u < WU; u += NW)
-            if (u + wave < WU)
-                to_lds(gw + (u + wave) * 1024, lw + (u + wave) * 1024, lane, WR - (u + wave) * 1024);
+        for (int u0 = 0; u0 < U; u0 += NW) {
+            const int u = u0 + wave;
+            if (u0 + NW > U && u >= U) break;
+            to_lds(u < XU ? gx + u * 1024 : gw + (u - XU) * 1024, lds + u * 1024, lane);
+        }
+        xj = a.list ? a.list[min(j + 1, j1 - 1)] - a.list0 : j + 1;
         __builtin_amdgcn_s_waitcnt(0x0f70);                   // vmcnt(0): the records are in LDS
+        xj = __builtin_amdgcn_readfirstlane(xj);
         __syncthreads();
+        const uint8_t *lx = lds, *lw = lds + XR;
         i8 w[TN];
         int ws[TN];
 #pragma unroll
@@ -314,10 +383,10 @@ __global__ __launch_bounds__(128 * WM, WFMT == kE2M1 ? 2 : 1) void k_gemm(const 
         __syncthreads();
     }
 
-    const int col0 = nbw * 256 + wn * 128 + 4 * (lane >> 4);   // outputs col0 + 16 n + r
+    const int col0 = (nbw * kWTiles + wn * TN) * 16 + 4 * (lane >> 4);   // outputs col0 + 16 n + r
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-        const int m = mb * BM + (wm * TM + i) * 16 + (lane & 15);
+        const int m = (mb * MT + wm * TM + i) * 16 + (lane & 15);
         if constexpr (EPI == kStore || EPI == kGrad) {
             if (m < a.M) {
                 float* y = a.y + (size_t)z * a.stride + (size_t)m * a.ld;
@@ -341,46 +410,236 @@ __global__ __launch_bounds__(128 * WM, WFMT == kE2M1 ? 2 : 1) void k_gemm(const 
             }
         } else if constexpr (EPI == kStats) {
             const int t = m < a.M ? a.targets[m] : -1;
-            float top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < TN; n++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int c = col0 + 16 * n + r;
-                    if (c >= a.N) acc[i][n][r] = -INFINITY;
-                    else if (c == t) a.zt[m] = acc[i][n][r];
-                    top = fmaxf(top, acc[i][n][r]);
-                }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // nothing above -inf: the sum is 0, or NaN where a logit is
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
-#pragma unroll
-            for (int n = 0; n < TN; n++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) sum += expf(acc[i][n][r] - ref);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (m < a.M && lane < 16)
-                a.part[(size_t)m * (2 * a.nbs) + 2 * nb + wn] = make_float2(top, sum);
+            const float2 o = stats<TN>(acc[i], col0, a.N, t, a.zt + m);
+            if (m < a.M && lane < 16) a.part[(size_t)m * (a.nbs * WN) + nb * WN + wn] = o;
         } else {
             // p = exp(z - lse) - [target]; rows past M and ignored ones are 0
             const int t = m < a.M ? a.targets[m] : -1;
             const bool live = t >= 0 && t < a.N;
             const float lse = live ? a.lse[m] : 0.0f;
-            float v[32];
+            Block v;
             probs(v, acc[i], col0, a.N, t, live, lse);
             const int mt = mb * MT + wm * TM + i;
             if (mt < a.pmt * a.pmbs) {
                 using P = Rows<CGX_MX_FP32>;
-                uint8_t* rec = a.p + ((size_t)(mt / a.pmt) * a.pk + 2 * nb + wn) *
-                                         (size_t)(a.pmt * (P::tile + 64));
+                uint8_t* rec = a.p + ((size_t)(mt / a.pmt) * a.pk + nb * WN + wn) * a.precord;
                 const int at = mt % a.pmt;
-                put<CGX_MX_FP32>(rec + at * P::tile, rec + a.pmt * P::tile + at * 64, lane,
-                                 cut<CGX_MX_FP32>(v));
+                put<CGX_MX_FP32>(rec + at * P::tile, rec + a.pmt * P::tile + at * 64, lane, v);
             }
         }
+    }
+}
+
+// Up to 16 rows: bound by the weight's bytes.  A block takes 16 T outputs at a
+// time and its waves the chunks of the contraction in turn, operands of the
+// weight going from memory to registers D chunks ahead.  The block cuts the
+// rows once, a lane a block of 32 (cutting them in the lanes that multiply them
+// would do M rows' work 16 / M times), into LDS without the rows that do not
+// exist; where they do not fit, a segment of the chunks at a time.  The waves'
+// sums meet in LDS.  At most a block a CU: where the outputs are more, a block
+// keeps its rows and goes on with the next ones, whose first operands are on
+// their way while it joins its waves' sums.
+struct Gemv {
+    const float* x;
+    size_t ldx;
+    int vecx;
+    const uint8_t* w;
+    int M, K, N, kc;
+    int tiles;             // of 16 outputs
+    int seg;               // chunks cut at a time (gemv_seg)
+    float* y;
+    size_t ld;
+    int vec;
+    const int* targets;
+    float2* part;          // [m][groups of T tiles]
+    float* zt;
+};
+constexpr int kGemvWaves = 8, kGemvAhead = 2;
+// bytes of a row's chunk in LDS
+template <int ACT>
+constexpr int gemv_chunk() { return 4 * (Rows<ACT>::terms * (ACT == CGX_MX_FP4 ? 16 : 24) + 1); }
+constexpr int kGemvLds = 152 << 10;
+constexpr int kGemvRound = kGemvAhead * kGemvWaves;    // chunks that the waves hold operands of
+static_assert((kGemvRound + 1) * 16 * gemv_chunk<CGX_MX_FP32>() <= kGemvLds, "a segment fits");
+// Chunks of a segment: all, or whole rounds.  An odd number of them is held.
+template <int ACT>
+int gemv_seg(int M, int kc) {
+    const int fit = kGemvLds / (M * gemv_chunk<ACT>());
+    return fit >= (kc | 1) ? kc : (fit - 1) / kGemvRound * kGemvRound;
+}
+
+template <int ACT, int T, int EPI>
+__global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
+    using R = Rows<ACT>;
+    constexpr bool six = ACT != CGX_MX_FP4;
+    constexpr int D = kGemvAhead, kRed = kGemvWaves * T * 1024;
+    static_assert(kRed <= kGemvLds && T <= kGemvWaves, "the waves' sums fit");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kGemvLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const unsigned l1 = lane, l16 = lane * 16;
+    // in LDS: 16 bytes of a block [term][row][block], the 8 others, the scales; an odd
+    // number of chunks a row, so that 16 rows' reads of one chunk spread over the banks
+    const int ld = 4 * (a.seg | 1), n16 = R::terms * a.M * ld;
+    uint8_t *const l8 = lds + n16 * 16, *const ls = l8 + (six ? n16 * 8 : 0);
+    // the rows stay where the waves' sums fit behind them
+    const int behind = (n16 * (six ? 24 : 16) + a.M * ld + 15) & ~15;
+    const bool stay = a.seg == a.kc && behind + kRed <= kGemvLds;
+    f4* red = (f4*)(lds + (stay ? behind : 0));
+    i4 q[D][T];
+    int s[D][T];
+    auto fetch = [&](int group, int c, i4* q, int* s) {
+        c = min(c, a.kc - 1);                                 // past the end: not used
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            // tiles past the last repeat it
+            const int tile = min(group * T + t, a.tiles - 1), at = tile & 15;
+            global_bytes p = (global_bytes)a.w + ((size_t)(tile >> 4) * a.kc + c) * kWRecord;
+            global_bytes codes = p + at * 1024, scale = p + kWTiles * 1024 + at * 64;
+            // kept in scalar registers: with the lane's part added ahead of time the
+            // addresses took 48 vector registers
+            asm volatile("" : "+s"(codes), "+s"(scale));
+            q[t] = *(const __attribute__((address_space(1))) i4*)(codes + l16);
+            s[t] = scale[l1];
+        }
+    };
+    // lanes past the last row repeat it: their products go nowhere
+    const int row = min(r, a.M - 1), groups = (a.tiles + T - 1) / T;
+    int group = blockIdx.x;
+#pragma unroll
+    for (int d = 0; d < D; d++) fetch(group, wave + d * kGemvWaves, q[d], s[d]);
+    for (bool fresh = true;; fresh = !stay) {
+        f4 acc[T];
+#pragma unroll
+        for (int t = 0; t < T; t++) acc[t] = f4{0, 0, 0, 0};
+        for (int c0 = 0; c0 < a.kc; c0 += a.seg) {
+            const int n = min(a.seg, a.kc - c0), blocks = 4 * n, total = a.M * blocks;
+            const bool vec = a.vecx && c0 * 128 + blocks * 32 <= a.K;
+            if (c0) __syncthreads();                          // the last segment is multiplied
+            if (fresh)
+                for (int u0 = wave * 64; u0 < total; u0 += 64 * kGemvWaves) {
+                    // lanes past the end repeat the last block
+                    const int u = min(u0 + lane, total - 1), m = u / blocks, b = u - m * blocks;
+                    Block x;
+                    load_block(x, a.x + (size_t)m * a.ldx, c0 * 128 + b * 32, a.K, vec);
+                    const int top = cut<ACT>(x, [&](int t, i8 v) {
+                        const int at = (t * a.M + m) * ld + b;
+                        *(i4*)(lds + at * 16) = i4{v[0], v[1], v[2], v[3]};
+                        if constexpr (six) *(i2*)(l8 + at * 8) = i2{v[4], v[5]};
+                    });
+                    ls[m * ld + b] = (uint8_t)top;
+                }
+            __syncthreads();
+            for (int c = wave; c < n; c += kGemvRound)
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    const int e = c + d * kGemvWaves;
+                    if (d && e >= n) break;
+                    const int top = ls[row * ld + 4 * e + g];
+#pragma unroll
+                    for (int t = 0; t < R::terms; t++) {
+                        const int at = (t * a.M + row) * ld + 4 * e + g;
+                        const i4 u = *(const i4*)(lds + at * 16);
+                        i8 x = {u[0], u[1], u[2], u[3], 0, 0, 0, 0};
+                        if constexpr (six) {
+                            const i2 v = *(const i2*)(l8 + at * 8);
+                            x[4] = v[0];
+                            x[5] = v[1];
+                        }
+#pragma unroll
+                        for (int k = 0; k < T; k++)
+                            acc[k] = mfma<kE2M1, R::fmt>(
+                                i8{q[d][k][0], q[d][k][1], q[d][k][2], q[d][k][3], 0, 0, 0, 0}, x,
+                                acc[k], s[d][k], top - term_shift(t));
+                    }
+                    if (c0 + e + kGemvRound < a.kc) fetch(group, c0 + e + kGemvRound, q[d], s[d]);
+                }
+        }
+        const int next = group + (int)gridDim.x;
+        if (next < groups)
+#pragma unroll
+            for (int d = 0; d < D; d++) fetch(next, wave + d * kGemvWaves, q[d], s[d]);
+        if (!stay) __syncthreads();                           // the rows are multiplied
+#pragma unroll
+        for (int t = 0; t < T; t++) red[(wave * T + t) * 64 + lane] = acc[t];
+        __syncthreads();
+        auto sum = [&](int t) {
+            f4 v = red[t * 64 + lane];
+#pragma unroll
+            for (int w = 1; w < kGemvWaves; w++) v += red[(w * T + t) * 64 + lane];
+            return v;
+        };
+        const int col = group * T * 16 + 4 * g;
+        if constexpr (EPI == kStore) {
+            for (int t = wave; t < T; t += kGemvWaves) {
+                const f4 v = sum(t);
+                const int n = col + 16 * t;
+                if (r >= a.M) continue;
+                float* y = a.y + (size_t)r * a.ld + n;
+                if (a.vec && n + 3 < a.N) {
+                    *(f4*)y = v;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (n + k < a.N) y[k] = v[k];
+                }
+            }
+        } else {
+            // a wave a tile, then a lane a row
+            const int t = r < a.M ? a.targets[r] : -1;
+            f4 v = {0, 0, 0, 0};
+            float2 o = {0, 0};
+            if (wave < T) {
+                v = sum(wave);
+                o = stats<1>(&v, col + 16 * wave, a.N, t, a.zt + r);
+            }
+            __syncthreads();
+            float2* tile = (float2*)red;
+            if (wave < T && lane < 16) tile[wave * 16 + lane] = o;
+            __syncthreads();
+            if (wave == 0 && lane < 16 && r < a.M) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < T; k++) top = fmaxf(top, tile[k * 16 + lane].x);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                float all = 0.0f;
+#pragma unroll
+                for (int k = 0; k < T; k++) {
+                    const float2 p = tile[k * 16 + lane];
+                    // a tile without a value above -inf holds 0, or NaN
+                    all += p.x == -INFINITY ? p.y : p.y * expf(p.x - ref);
+                }
+                a.part[(size_t)r * groups + group] = make_float2(top, all);
+            }
+        }
+        if (next >= groups) return;
+        group = next;
+        __syncthreads();                                      // the sums are read
+    }
+}
+
+// Tiles a block: the fewest that leave at most a block a CU, up to eight.  One
+// block a CU and more tiles beat more blocks, each of which cuts the rows: one
+// row through 4096 x 22016 10.3 us with 6 tiles (230 blocks), 13.2 with 3.
+inline int gemv_tiles(int tiles) {
+    for (int t : {1, 2, 3, 4, 6})
+        if (tiles <= 256 * t) return t;
+    return 8;
+}
+inline int gemv_groups(int tiles) { return (tiles + gemv_tiles(tiles) - 1) / gemv_tiles(tiles); }
+
+template <int ACT, int EPI>
+void gemv_launch(Gemv g, hipStream_t st) {
+    g.seg = gemv_seg<ACT>(g.M, g.kc);
+    const int groups = gemv_groups(g.tiles);
+    const dim3 grid(groups < 256 ? groups : 256), block(64 * kGemvWaves);
+    switch (gemv_tiles(g.tiles)) {
+        case 1: hipLaunchKernelGGL((k_gemv<ACT, 1, EPI>), grid, block, 0, st, g); break;
+        case 2: hipLaunchKernelGGL((k_gemv<ACT, 2, EPI>), grid, block, 0, st, g); break;
+        case 3: hipLaunchKernelGGL((k_gemv<ACT, 3, EPI>), grid, block, 0, st, g); break;
+        case 4: hipLaunchKernelGGL((k_gemv<ACT, 4, EPI>), grid, block, 0, st, g); break;
+        case 6: hipLaunchKernelGGL((k_gemv<ACT, 6, EPI>), grid, block, 0, st, g); break;
+        default: hipLaunchKernelGGL((k_gemv<ACT, 8, EPI>), grid, block, 0, st, g);
     }
 }
 

@@ -66,6 +66,7 @@ constexpr size_t kPiece = (size_t)128 << 20;       // bytes of a piece's probabi
 struct Plan {
     int mt, mbs, nbs;            // the product over the vocabulary
     size_t rows, part, zt;       // bytes
+    int parts;                   // of a row's sums
     int mt2, mbs2, kbs, piece;   // the second product; chunks of a piece
     size_t p, sum;
 };
@@ -74,16 +75,22 @@ int splits_of(const Plan& p, int chunks) {
 }
 Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
     Plan p = {};
-    p.mt = cgk_mx_tiles(M);
-    p.mbs = up(M, 16 * p.mt);
-    p.nbs = up(w->N, 256);
-    p.rows = whole(cgk_mx_rows_bytes(M, w->K, act, p.mt));
-    if (!grad) {
-        p.part = whole((size_t)M * 2 * p.nbs * sizeof(float2));
-        p.zt = whole((size_t)M * 4);
+    p.zt = grad ? 0 : whole((size_t)M * 4);
+    if (!grad && M <= 16) {      // k_gemv
+        p.parts = gemv_groups(up(w->N, 16));
+        p.part = whole((size_t)M * p.parts * sizeof(float2));
         return p;
     }
-    p.mt2 = std::min(p.mt, 4);
+    p.mt = cgk_mx_tiles(M, w->N, act);
+    p.mbs = up(M, 16 * p.mt);
+    p.nbs = up(w->N, 256);
+    p.parts = 2 * p.nbs;
+    p.rows = whole(cgk_mx_rows_bytes(M, w->K, act, p.mt));
+    if (!grad) {
+        p.part = whole((size_t)M * p.parts * sizeof(float2));
+        return p;
+    }
+    p.mt2 = M <= 32 ? 2 : 4;
     p.mbs2 = up(M, 16 * p.mt2);
     p.kbs = up(w->K, 256);
     const size_t chunk = (size_t)p.mbs2 * rows_record<CGX_MX_FP32>(p.mt2);
@@ -102,10 +109,9 @@ size_t bytes(const Plan& p) { return p.rows + p.part + p.zt + p.p + p.sum; }
 template <int ACT, int EPI>
 void over_vocabulary(const Gemm& g, int mt) {
     const dim3 grid(g.mbs * g.nbs);
-    if (mt == 1) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 16, 1, EPI>), grid, dim3(128), 0, stream(), g);
-    else if (mt == 2) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 32, 1, EPI>), grid, dim3(128), 0, stream(), g);
-    else if (mt == 4) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 64, 1, EPI>), grid, dim3(128), 0, stream(), g);
-    else hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 128, 2, EPI>), grid, dim3(256), 0, stream(), g);
+    if (mt == 2) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 2, 2, EPI>), grid, dim3(256), 0, stream(), g);
+    else if (mt == 4) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 4, 2, EPI>), grid, dim3(256), 0, stream(), g);
+    else hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 8, 2, EPI>), grid, dim3(256), 0, stream(), g);
 }
 template <int EPI>
 int over_vocabulary(const Gemm& g, int mt, int act) {
@@ -117,9 +123,8 @@ int over_vocabulary(const Gemm& g, int mt, int act) {
 template <int EPI>
 int over_inputs(const Gemm& g, int mt) {
     const dim3 grid(g.mbs * g.nbs, g.splits);
-    if (mt == 1) hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 16, 1, EPI>), grid, dim3(128), 0, stream(), g);
-    else if (mt == 2) hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 32, 1, EPI>), grid, dim3(128), 0, stream(), g);
-    else hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 64, 1, EPI>), grid, dim3(128), 0, stream(), g);
+    if (mt == 2) hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 2, 2, EPI>), grid, dim3(256), 0, stream(), g);
+    else hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 4, 2, EPI>), grid, dim3(256), 0, stream(), g);
     return launch_check("mx loss gradient");
 }
 
@@ -164,12 +169,33 @@ extern "C" int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight
         uint8_t* rows = (uint8_t*)ws;
         float2* part = (float2*)(rows + p.rows);
         float* zt = (float*)((uint8_t*)part + p.part);
-        if (cgk_mx_rows(x + (size_t)m0 * ld, ld, m, w->K, act, p.mt, rows)) return -1;
-        Gemm g = logits(w, rows, p, m, targets + m0);
-        g.part = part;
-        g.zt = zt;
-        if (over_vocabulary<kStats>(g, p.mt, act)) return -1;
-        hipLaunchKernelGGL(k_loss, dim3(up(m, 4)), dim3(256), 0, stream(), part, 2 * p.nbs, zt,
+        const float* xm = x + (size_t)m0 * ld;
+        if (m <= 16) {
+            Gemv g = {};
+            g.x = xm;
+            g.ldx = ld;
+            g.vecx = ((uintptr_t)xm & 15) == 0 && ld % 4 == 0;
+            g.w = w->codes;
+            g.M = m;
+            g.K = w->K;
+            g.N = w->N;
+            g.kc = up(w->K, 128);
+            g.tiles = up(w->N, 16);
+            g.targets = targets + m0;
+            g.part = part;
+            g.zt = zt;
+            if (act == CGX_MX_FP4) gemv_launch<CGX_MX_FP4, kStats>(g, stream());
+            else if (act == CGX_MX_FP6) gemv_launch<CGX_MX_FP6, kStats>(g, stream());
+            else gemv_launch<CGX_MX_FP32, kStats>(g, stream());
+            if (launch_check("mx loss of few rows")) return -1;
+        } else {
+            if (cgk_mx_rows(xm, ld, m, w->K, act, p.mt, rows)) return -1;
+            Gemm g = logits(w, rows, p, m, targets + m0);
+            g.part = part;
+            g.zt = zt;
+            if (over_vocabulary<kStats>(g, p.mt, act)) return -1;
+        }
+        hipLaunchKernelGGL(k_loss, dim3(up(m, 4)), dim3(256), 0, stream(), part, p.parts, zt,
                            targets + m0, m, w->N, loss ? loss + m0 : nullptr,
                            lse ? lse + m0 : nullptr);
         if (launch_check("mx loss join")) return -1;
@@ -198,6 +224,7 @@ extern "C" int cgk_mx_loss_grad(const float* x, size_t ld, int M, const cgx_mx_w
             g.pk = p.piece;
             g.pmt = p.mt2;
             g.pmbs = p.mbs2;
+            g.precord = rows_record<CGX_MX_FP32>(p.mt2);
             if (over_vocabulary<kProbs>(g, p.mt, act)) return -1;
             Gemm t = {};
             t.x = probs;
