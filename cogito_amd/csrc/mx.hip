@@ -22,20 +22,34 @@ int launch_check(const char* what) {
 inline int up(long long a, int b) { return (int)((a + b - 1) / b); }
 
 // ------------------------------------------------- quantise and read back
+// Eight values of a row from k on, 0 past its end.
+__device__ __forceinline__ void load8(float* v, const float* x, int k, int cols) {
+    if (k + 8 <= cols) {
+        const f4 a = *(const f4u*)(x + k), b = *(const f4u*)(x + k + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? x[k + i] : 0.0f;
+    }
+}
+
 // Four lanes a block, eight values each; a wave takes 16 blocks of one row.
 // The 6-bit conversion takes 32 values: a lane's eight go first and their six
 // bytes are kept.
 template <int FMT>
 __global__ __launch_bounds__(256) void k_quantize(const float* __restrict__ x, size_t ld, int rows,
-                                                  int cols, int segs, bool vec,
-                                                  uint8_t* __restrict__ codes,
+                                                  int cols, int segs, uint8_t* __restrict__ codes,
                                                   uint8_t* __restrict__ scales) {
     const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int row = wave / segs, seg = wave - row * segs, blocks = (cols + 31) / 32;
     if (row >= rows) return;
     const int lane = threadIdx.x & 63, blk = seg * 16 + (lane >> 2), part = lane & 3;
     float v[8];
-    load8(v, x + (size_t)row * ld, blk * 32 + part * 8, cols, vec);
+    load8(v, x + (size_t)row * ld, blk * 32 + part * 8, cols);
     int top = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -88,8 +102,7 @@ __device__ __forceinline__ float value6(int q) {
 template <int FMT>
 __global__ __launch_bounds__(256) void k_dequantize(const uint8_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, int rows,
-                                                    int cols, int segs, bool vec,
-                                                    float* __restrict__ y, size_t ld) {
+                                                    int cols, int segs, float* __restrict__ y, size_t ld) {
     const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int row = wave / segs, seg = wave - row * segs, blocks = (cols + 31) / 32;
     const int lane = threadIdx.x & 63, blk = seg * 16 + (lane >> 2), part = lane & 3;
@@ -110,9 +123,9 @@ __global__ __launch_bounds__(256) void k_dequantize(const uint8_t* __restrict__ 
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = byte == 255 ? NAN : ldexpf(v[i], byte - 127);
     float* o = y + (size_t)row * ld + k;
-    if (vec && k + 8 <= cols) {
-        *(f4*)o = f4{v[0], v[1], v[2], v[3]};
-        *(f4*)(o + 4) = f4{v[4], v[5], v[6], v[7]};
+    if (k + 8 <= cols) {
+        *(f4u*)o = f4{v[0], v[1], v[2], v[3]};
+        *(f4u*)(o + 4) = f4{v[4], v[5], v[6], v[7]};
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -247,7 +260,7 @@ __global__ __launch_bounds__(256) void k_transposed(const uint8_t* __restrict__ 
 // A wave a tile of 16 rows and a chunk, a lane a block.
 template <int ACT>
 __global__ __launch_bounds__(256) void k_rows(const float* __restrict__ x, size_t ld, int M, int K,
-                                              int kc, int mt, long long units, bool vec,
+                                              int kc, int mt, long long units,
                                               uint8_t* __restrict__ out) {
     const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (u >= units) return;
@@ -255,38 +268,53 @@ __global__ __launch_bounds__(256) void k_rows(const float* __restrict__ x, size_
     // rows past the last repeat it: nothing of theirs is stored
     const int m = min(tile * 16 + (lane & 15), M - 1);
     Block v;
-    load_block(v, x + (size_t)m * ld, c * 128 + (lane >> 4) * 32, K, vec && c * 128 + 128 <= K);
+    load_block(v, x + (size_t)m * ld, c * 128 + (lane >> 4) * 32, K, c * 128 + 128 <= K);
     using R = Rows<ACT>;
     const int b = tile / mt, at = tile - b * mt;
     uint8_t* rec = out + ((size_t)b * kc + c) * (size_t)rows_record<ACT>(mt);
     put<ACT>(rec + at * R::tile, rec + mt * R::tile + at * 64, lane, v);
 }
 
-// Splits of a product in order: y[m][n] (+)= row_scale[m] * sum of part[s][m][n];
-// 0 in a row whose target is none of V.
+// Splits of a product: y[m][n] (+)= row_scale[m] * sum of part[s][m][n], 0 in a
+// row whose target is none of V.  G lanes take the splits of four outputs in
+// turn, four loads in flight, and their sums are added in order: 49 splits of
+// 61 x 768 with one lane ... us, with eight ....
+template <int G>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int splits,
                                               size_t stride, int pld, int M, int N,
-                                              float* __restrict__ y, size_t ld, bool vec,
+                                              float* __restrict__ y, size_t ld,
                                               const float* __restrict__ row_scale,
                                               const int* __restrict__ targets, int V, int add) {
-    const int q = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y, n = 4 * q;
-    if (n >= N) return;
-    const float* p = part + (size_t)m * pld + n;
+    constexpr int Q = 256 / G;                                // fours of outputs
+    __shared__ f4 sum[G][Q];
+    const int q = threadIdx.x % Q, g = threadIdx.x / Q, m = blockIdx.y;
+    const int n = 4 * (blockIdx.x * Q + q);
     f4 v = {0, 0, 0, 0};
-    for (int s = 0; s < splits; s += 8) {
-        f4 t[8];
+    if (n < N) {
+        const float* p = part + (size_t)m * pld + n;
+        for (int s = g; s < splits; s += 4 * G) {
+            f4 t[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = *(const f4*)(p + (size_t)min(s + i, splits - 1) * stride);
+            for (int i = 0; i < 4; i++) t[i] = *(const f4*)(p + (size_t)min(s + G * i, splits - 1) * stride);
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (s + i < splits) v += t[i];
+            for (int i = 0; i < 4; i++)
+                if (s + G * i < splits) v += t[i];
+        }
     }
+    if constexpr (G > 1) {
+        sum[g][q] = v;
+        __syncthreads();
+        if (g) return;
+#pragma unroll
+        for (int i = 1; i < G; i++) v += sum[i][q];
+    }
+    if (n >= N) return;
     if (row_scale) v *= row_scale[m];
     if (targets && (unsigned)targets[m] >= (unsigned)V) v = f4{0, 0, 0, 0};
     float* o = y + (size_t)m * ld + n;
-    if (vec && n + 3 < N) {
-        if (add) v += *(const f4*)o;
-        *(f4*)o = v;
+    if (n + 3 < N) {
+        if (add) v += *(const f4u*)o;
+        *(f4u*)o = v;
     } else {
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -300,28 +328,26 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
 extern "C" int cgk_mx_quantize(const float* x, size_t ld, int rows, int cols, int format,
                                uint8_t* codes, uint8_t* scales) {
     const int segs = up(cols, 512);
-    const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0;
     const dim3 grid(up((long long)rows * segs, 4));
     if (format == CGX_MX_FP4)
         hipLaunchKernelGGL((k_quantize<CGX_MX_FP4>), grid, dim3(256), 0, stream(), x, ld, rows, cols,
-                           segs, vec, codes, scales);
+                           segs, codes, scales);
     else
         hipLaunchKernelGGL((k_quantize<CGX_MX_FP6>), grid, dim3(256), 0, stream(), x, ld, rows, cols,
-                           segs, vec, codes, scales);
+                           segs, codes, scales);
     return launch_check("mx quantize");
 }
 
 extern "C" int cgk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int cols,
                                  int format, float* y, size_t ld) {
     const int segs = up(cols, 512);
-    const bool vec = ((uintptr_t)y & 15) == 0 && ld % 4 == 0;
     const dim3 grid(up((long long)rows * segs, 4));
     if (format == CGX_MX_FP4)
         hipLaunchKernelGGL((k_dequantize<CGX_MX_FP4>), grid, dim3(256), 0, stream(), codes, scales,
-                           rows, cols, segs, vec, y, ld);
+                           rows, cols, segs, y, ld);
     else
         hipLaunchKernelGGL((k_dequantize<CGX_MX_FP6>), grid, dim3(256), 0, stream(), codes, scales,
-                           rows, cols, segs, vec, y, ld);
+                           rows, cols, segs, y, ld);
     return launch_check("mx dequantize");
 }
 
@@ -361,10 +387,9 @@ extern "C" int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list
 extern "C" int cgk_mx_rows(const float* x, size_t ld, int M, int K, int act, int mt, uint8_t* out) {
     const int kc = up(K, 128);
     const long long units = (long long)up(M, 16 * mt) * mt * kc;
-    const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0;
     const dim3 grid(up(units, 4));
     auto go = [&](auto k) {
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, stream(), x, ld, M, K, kc, mt, units, vec, out);
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, stream(), x, ld, M, K, kc, mt, units, out);
     };
     if (act == CGX_MX_FP4) go(k_rows<CGX_MX_FP4>);
     else if (act == CGX_MX_FP6) go(k_rows<CGX_MX_FP6>);
@@ -380,9 +405,12 @@ extern "C" size_t cgk_mx_rows_bytes(int M, int K, int act, int mt) {
 extern "C" int cgk_mx_join(const float* part, int splits, size_t stride, int pld, int M, int N,
                            float* y, size_t ld, const float* row_scale, const int* targets,
                            int V, int add) {
-    const bool vec = ((uintptr_t)y & 15) == 0 && ld % 4 == 0;
-    hipLaunchKernelGGL(k_join, dim3(up(N, 1024), M), dim3(256), 0, stream(), part, splits, stride,
-                       pld, M, N, y, ld, vec, row_scale, targets, V, add);
+    if (splits > 4)
+        hipLaunchKernelGGL((k_join<8>), dim3(up(N, 128), M), dim3(256), 0, stream(), part, splits,
+                           stride, pld, M, N, y, ld, row_scale, targets, V, add);
+    else
+        hipLaunchKernelGGL((k_join<1>), dim3(up(N, 1024), M), dim3(256), 0, stream(), part, splits,
+                           stride, pld, M, N, y, ld, row_scale, targets, V, add);
     return launch_check("mx join");
 }
 
@@ -403,7 +431,8 @@ Plan plan(const cgx_mx_weight* w, int M, int act) {
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
     const int kc = up(w->K, 128), blocks = p.mbs * p.nbs;
-    p.splits = std::max(1, std::min(512 / blocks, kc / 4));
+    // a join costs what four or five chunks of a block do
+    p.splits = std::max(1, std::min(512 / blocks, kc < 16 ? 1 : kc / 4));
     p.rows = (cgk_mx_rows_bytes(M, w->K, act, p.mt) + 255) & ~(size_t)255;
     p.part = p.splits > 1 ? (size_t)p.splits * M * ((w->N + 3) & ~3) * 4 : 0;
     return p;
@@ -466,7 +495,6 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
             Gemv g = {};
             g.x = xm;
             g.ldx = ldx;
-            g.vecx = ((uintptr_t)xm & 15) == 0 && ldx % 4 == 0;
             g.w = w->codes;
             g.M = m;
             g.K = w->K;
@@ -474,7 +502,6 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
             g.kc = up(w->K, 128);
             g.y = ym;
             g.ld = ldy;
-            g.vec = ((uintptr_t)ym & 15) == 0 && ldy % 4 == 0;
             g.tiles = up(w->N, 16);
             if (act == CGX_MX_FP4) gemv<CGX_MX_FP4>(g);
             else if (act == CGX_MX_FP6) gemv<CGX_MX_FP6>(g);
@@ -498,11 +525,9 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
             g.y = (float*)(rows + p.rows);
             g.ld = pld;
             g.stride = (size_t)m * pld;
-            g.vec = 1;
         } else {
             g.y = ym;
             g.ld = ldy;
-            g.vec = ((uintptr_t)ym & 15) == 0 && ldy % 4 == 0;
         }
         if (act == CGX_MX_FP4) gemm<CGX_MX_FP4>(g, p.mt);
         else if (act == CGX_MX_FP6) gemm<CGX_MX_FP6>(g, p.mt);

@@ -28,7 +28,7 @@ typedef int i2 __attribute__((ext_vector_type(2)));
 typedef int i8 __attribute__((ext_vector_type(8)));
 typedef unsigned u6 __attribute__((ext_vector_type(6)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // rows start anywhere
 typedef float f16 __attribute__((ext_vector_type(16)));
 typedef float f32 __attribute__((ext_vector_type(32)));
 
@@ -151,28 +151,14 @@ __device__ __forceinline__ void put(uint8_t* tile, uint8_t* sc, int lane, Block&
     });
 }
 
-// Eight values of a row from k on, 0 past its end.
-__device__ __forceinline__ void load8(float* v, const float* x, int k, int cols, bool vec) {
-    if (vec && k + 8 <= cols) {
-        const f4 a = *(const f4*)(x + k), b = *(const f4*)(x + k + 4);
+// The block from value k of a row on, 0 past the row's end.  whole: every
+// lane's block lies within its row; the loads go to where the conversion reads,
+// so that they stay in flight until then.
+__device__ __forceinline__ void load_block(Block& b, const float* x, int k, int cols, bool whole) {
+    if (whole) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? x[k + i] : 0.0f;
-    }
-}
-// The block from value k of a row on, 0 past the row's end.  vec: every lane's
-// block lies within 16-byte aligned rows; the loads go to where the conversion
-// reads, so that they stay in flight until then.
-__device__ __forceinline__ void load_block(Block& b, const float* x, int k, int cols, bool vec) {
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const f4 v = *(const f4*)(x + k + 4 * i), w = *(const f4*)(x + k + 16 + 4 * i);
+            const f4 v = *(const f4u*)(x + k + 4 * i), w = *(const f4u*)(x + k + 16 + 4 * i);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 b.a[4 * i + j] = v[j];
@@ -227,7 +213,6 @@ struct Gemm {
     // store: y[split][m][n] (rows ld apart, splits `stride` apart)
     float* y;
     size_t ld, stride;
-    int vec;               // y takes 16-byte stores
     // gradient: y (+)= row_scale[m] * sum, 0 in a row whose target is none of V
     const float* row_scale;
     const int* targets;
@@ -397,9 +382,9 @@ __global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 
                     const int c = col0 + 16 * n;
                     f4 v = EPI == kGrad ? acc[i][n] * g : acc[i][n];
                     if (none) v = f4{0, 0, 0, 0};
-                    if (a.vec && c + 3 < a.N) {
-                        if (EPI == kGrad && a.add) v += *(const f4*)(y + c);
-                        *(f4*)(y + c) = v;
+                    if (c + 3 < a.N) {
+                        if (EPI == kGrad && a.add) v += *(const f4u*)(y + c);
+                        *(f4u*)(y + c) = v;
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; r++)
@@ -442,14 +427,12 @@ __global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 
 struct Gemv {
     const float* x;
     size_t ldx;
-    int vecx;
     const uint8_t* w;
     int M, K, N, kc;
     int tiles;             // of 16 outputs
     int seg;               // chunks cut at a time (gemv_seg)
     float* y;
     size_t ld;
-    int vec;
     const int* targets;
     float2* part;          // [m][groups of T tiles]
     float* zt;
@@ -514,14 +497,14 @@ __global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
         for (int t = 0; t < T; t++) acc[t] = f4{0, 0, 0, 0};
         for (int c0 = 0; c0 < a.kc; c0 += a.seg) {
             const int n = min(a.seg, a.kc - c0), blocks = 4 * n, total = a.M * blocks;
-            const bool vec = a.vecx && c0 * 128 + blocks * 32 <= a.K;
+            const bool whole = c0 * 128 + blocks * 32 <= a.K;
             if (c0) __syncthreads();                          // the last segment is multiplied
             if (fresh)
                 for (int u0 = wave * 64; u0 < total; u0 += 64 * kGemvWaves) {
                     // lanes past the end repeat the last block
                     const int u = min(u0 + lane, total - 1), m = u / blocks, b = u - m * blocks;
                     Block x;
-                    load_block(x, a.x + (size_t)m * a.ldx, c0 * 128 + b * 32, a.K, vec);
+                    load_block(x, a.x + (size_t)m * a.ldx, c0 * 128 + b * 32, a.K, whole);
                     const int top = cut<ACT>(x, [&](int t, i8 v) {
                         const int at = (t * a.M + m) * ld + b;
                         *(i4*)(lds + at * 16) = i4{v[0], v[1], v[2], v[3]};
@@ -576,8 +559,8 @@ __global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
                 const int n = col + 16 * t;
                 if (r >= a.M) continue;
                 float* y = a.y + (size_t)r * a.ld + n;
-                if (a.vec && n + 3 < a.N) {
-                    *(f4*)y = v;
+                if (n + 3 < a.N) {
+                    *(f4u*)y = v;
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; k++)

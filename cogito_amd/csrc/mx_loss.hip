@@ -32,29 +32,43 @@ int launch_check(const char* what) {
 inline int up(long long a, int b) { return (int)((a + b - 1) / b); }
 inline size_t whole(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Joins the parts of a row: a wave a row.  Sums in double (a few values a lane).
+// Joins the parts of a row, a block a row: every part read once, its sum taken
+// to the larger maximum, in double (a few a thread).
+struct Sum {
+    float top;
+    double sum;
+};
+__device__ __forceinline__ Sum join(Sum a, Sum b) {
+    // a part without a value above -inf holds 0, or NaN
+    const float top = fmaxf(a.top, b.top), ref = top == -INFINITY ? 0.0f : top;
+    const float ea = a.top == -INFINITY ? 1.0f : expf(a.top - ref);
+    const float eb = b.top == -INFINITY ? 1.0f : expf(b.top - ref);
+    return {top, a.sum * ea + b.sum * eb};
+}
 __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, int parts,
                                               const float* __restrict__ zt,
-                                              const int* __restrict__ targets, int rows, int V,
+                                              const int* __restrict__ targets, int V,
                                               float* __restrict__ loss, float* __restrict__ lse) {
-    const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (m >= rows) return;
+    __shared__ Sum wave[4];
+    const int m = blockIdx.x, lane = threadIdx.x & 63;
     const float2* p = part + (size_t)m * parts;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, p[i].x);
+    Sum s = {-INFINITY, 0.0};
+    for (int i = threadIdx.x; i < parts; i += 1024) {
+        float2 q[4];
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    double sum = 0.0;
-    for (int i = lane; i < parts; i += 64) {
-        const float2 q = p[i];
-        // a part without a value above -inf holds 0, or NaN
-        sum += q.x == -INFINITY ? (double)q.y : (double)q.y * (double)expf(q.x - ref);
+        for (int j = 0; j < 4; j++)
+            q[j] = i + 256 * j < parts ? p[i + 256 * j] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s = join(s, Sum{q[j].x, q[j].y});
     }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane) return;
-    const double l = (double)ref + log(sum);
+    for (int o = 32; o; o >>= 1) s = join(s, Sum{__shfl_xor(s.top, o), __shfl_xor(s.sum, o)});
+    if (lane == 0) wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int w = 1; w < 4; w++) s = join(s, wave[w]);
+    const double l = (double)(s.top == -INFINITY ? 0.0f : s.top) + log(s.sum);
     const int t = targets[m];
     if (lse) lse[m] = (float)l;
     if (loss) loss[m] = t >= 0 && t < V ? (float)(l - (double)zt[m]) : 0.0f;
@@ -174,7 +188,6 @@ extern "C" int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight
             Gemv g = {};
             g.x = xm;
             g.ldx = ld;
-            g.vecx = ((uintptr_t)xm & 15) == 0 && ld % 4 == 0;
             g.w = w->codes;
             g.M = m;
             g.K = w->K;
@@ -195,8 +208,8 @@ extern "C" int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight
             g.zt = zt;
             if (over_vocabulary<kStats>(g, p.mt, act)) return -1;
         }
-        hipLaunchKernelGGL(k_loss, dim3(up(m, 4)), dim3(256), 0, stream(), part, p.parts, zt,
-                           targets + m0, m, w->N, loss ? loss + m0 : nullptr,
+        hipLaunchKernelGGL(k_loss, dim3(m), dim3(256), 0, stream(), part, p.parts, zt,
+                           targets + m0, w->N, loss ? loss + m0 : nullptr,
                            lse ? lse + m0 : nullptr);
         if (launch_check("mx loss join")) return -1;
     }
@@ -245,7 +258,6 @@ extern "C" int cgk_mx_loss_grad(const float* x, size_t ld, int M, const cgx_mx_w
                 t.y = sum;
                 t.ld = pld;
                 t.stride = (size_t)m * pld;
-                t.vec = 1;
                 if (over_inputs<kStore>(t, p.mt2) ||
                     cgk_mx_join(sum, t.splits, t.stride, pld, m, w->K, dm, ldd, scale,
                                 targets + m0, w->N, c > 0))
@@ -253,7 +265,6 @@ extern "C" int cgk_mx_loss_grad(const float* x, size_t ld, int M, const cgx_mx_w
             } else {
                 t.y = dm;
                 t.ld = ldd;
-                t.vec = ((uintptr_t)dm & 15) == 0 && ldd % 4 == 0;
                 t.row_scale = scale;
                 t.targets = targets + m0;
                 t.V = w->N;
