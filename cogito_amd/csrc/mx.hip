@@ -426,7 +426,7 @@ struct Plan {
 };
 Plan plan(const cgx_mx_weight* w, int M, int act) {
     Plan p = {};
-    if (M <= 16) return p;           // k_gemv
+    if (gemv_pays(M, w->K)) return p;
     p.mt = cgk_mx_tiles(M, w->N, act);
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
@@ -439,12 +439,7 @@ Plan plan(const cgx_mx_weight* w, int M, int act) {
 }
 
 template <int ACT>
-void gemm(const Gemm& g, int mt) {
-    const dim3 grid(g.mbs * g.nbs, g.splits);
-    if (mt == 2) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 2, 2, kStore>), grid, dim3(256), 0, stream(), g);
-    else if (mt == 4) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 4, 2, kStore>), grid, dim3(256), 0, stream(), g);
-    else hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 8, 2, kStore>), grid, dim3(256), 0, stream(), g);
-}
+void gemm(const Gemm& g, int mt) { gemm_launch<ACT, kE2M1, kStore>(g, mt, stream()); }
 template <int ACT>
 void gemv(const Gemv& g) {
     gemv_launch<ACT, kStore>(g, stream());
@@ -458,6 +453,7 @@ void gemv(const Gemv& g) {
 // (61 rows through 768 x 50257: 13.6 us with 32 rows, 15.4 with 64).
 extern "C" int cgk_mx_tiles(int M, int N, int act) {
     (void)act;
+    if (M <= 16) return 1;
     int mt = 10 * up(M, 128) * 128 <= 11 * up(M, 64) * 64 ? 8 : 4;
     while (mt > 2 && (long long)up(M, 16 * mt) * up(N, 256) < 512) mt /= 2;
     return mt;
@@ -491,7 +487,7 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
         const Plan p = plan(w, m, act);
         const float* xm = x + (size_t)m0 * ldx;
         float* ym = y + (size_t)m0 * ldy;
-        if (m <= 16) {
+        if (gemv_pays(m, w->K)) {
             Gemv g = {};
             g.x = xm;
             g.ldx = ldx;

@@ -199,6 +199,18 @@ __device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l, int lane) {
         (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
+typedef const __attribute__((address_space(4))) int* constant_ints;   // read by scalar loads
+
+// s_waitcnt's operand that waits until n of a wave's loads are outstanding
+constexpr int wait_loads(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
+
+// The block's waves meet; what the compiler moves over no side of it.
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // What a product's epilogue needs.
 struct Gemm {
     const uint8_t* x;      // records of the rows [row block][chunk]
@@ -305,15 +317,23 @@ __device__ __forceinline__ float2 stats(f4* v, int col, int N, int t, float* zt)
 
 // Product of 16 MT rows and 256 outputs a block of WM x 2 waves.  The weight's
 // tile is the first operand, so that a lane holds four neighbouring outputs of
-// one row.  A step takes a chunk; its records go into LDS without passing
-// registers.
-template <int ACT, int WFMT, int MT, int WM, int EPI>
-__global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 3 : 4) void k_gemm(const Gemm a) {
+// one row.  Records go into LDS without passing registers, PER chunks of the
+// contraction a step (more where a chunk is little work: one term).  The blocks
+// of a CU overlap one's copies with another's matrix instructions; a launch of
+// at most a block a CU (DEEP) copies the next chunk while it multiplies one,
+// into a second array, so that the compiler sees that reads of the first need
+// not wait for it.
+template <int ACT, int WFMT, int MT, int WM, int PER, bool DEEP, int EPI>
+__global__ __launch_bounds__(128 * WM, DEEP ? (WM + 1) / 2 : MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 3 : MT == 2 ? 4 : 2)
+void k_gemm(const Gemm a) {
     constexpr int WN = 2, TM = MT / WM, TN = kWTiles / WN, NW = WM * WN;
     using R = Rows<ACT>;
     constexpr int XR = rows_record<ACT>(MT), WT = WFMT == kE2M1 ? 1024 : 1536;
     constexpr int WR = WFMT == kE2M1 ? kWRecord : kTRecord, XU = XR / 1024, U = XU + WR / 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[XR + WR];
+    constexpr int COPIES = (U + NW - 1) / NW;                 // of a wave a chunk
+    static_assert(PER == 1 || !DEEP, "one chunk at a time");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PER * COPIES * NW * 1024];
+    __shared__ __attribute__((aligned(16))) uint8_t lds2[DEEP ? COPIES * NW * 1024 : 16];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // each XCD (block b runs on XCD b % 8) takes a run of outputs with all their rows
@@ -331,41 +351,69 @@ __global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f4{0, 0, 0, 0};
 
-    int xj = a.list ? a.list[j0] - a.list0 : j0;
-    for (int j = j0; j < j1; j++) {
-        const uint8_t* gx = xb + (size_t)xj * XR;
+    // every wave issues the same number of copies; those past the record repeat its last KiB
+    auto copy = [&](int j, uint8_t* l) {
+        const uint8_t* gx = xb + (size_t)(a.list ? ((constant_ints)a.list)[j] - a.list0 : j) * XR;
         const uint8_t* gw = wb + (size_t)j * WR;
 #pragma unroll
-        for (int u0 = 0; u0 < U; u0 += NW) {
-            const int u = u0 + wave;
-            if (u0 + NW > U && u >= U) break;
-            to_lds(u < XU ? gx + u * 1024 : gw + (u - XU) * 1024, lds + u * 1024, lane);
+        for (int i = 0; i < COPIES; i++) {
+            const int u = i * NW + wave, v = i == COPIES - 1 ? min(u, U - 1) : u;
+            to_lds(v < XU ? gx + v * 1024 : gw + (v - XU) * 1024, l + u * 1024, lane);
         }
-        xj = a.list ? a.list[min(j + 1, j1 - 1)] - a.list0 : j + 1;
-        __builtin_amdgcn_s_waitcnt(0x0f70);                   // vmcnt(0): the records are in LDS
-        xj = __builtin_amdgcn_readfirstlane(xj);
-        __syncthreads();
-        const uint8_t *lx = lds, *lw = lds + XR;
-        i8 w[TN];
-        int ws[TN];
+    };
+    auto multiply = [&](const uint8_t* lx) {
+        const uint8_t* lw = lx + XR;
+        __builtin_amdgcn_sched_barrier(0);
+        i8 w[TN], x = operand<R::fmt>(lx + wm * TM * R::tile, lane);
+        int ws[TN], xs[TM];
+#pragma unroll
+        for (int i = 0; i < TM; i++) xs[i] = lx[MT * R::tile + (wm * TM + i) * 64 + lane];
 #pragma unroll
         for (int n = 0; n < TN; n++) {
             w[n] = operand<WFMT>(lw + (wn * TN + n) * WT, lane);
             ws[n] = lw[kWTiles * WT + (wn * TN + n) * 64 + lane];
         }
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const uint8_t* t0 = lx + (wm * TM + i) * R::tile;
-            const int xs = lx[MT * R::tile + (wm * TM + i) * 64 + lane];
+        for (int q = 0; q < TM * R::terms; q++) {
+            const int i = q / R::terms, t = q % R::terms, p = q + 1;
+            i8 next = x;                                      // read ahead of this one's instructions
+            if (p < TM * R::terms)
+                next = operand<R::fmt>(lx + (wm * TM + p / R::terms) * R::tile + p % R::terms * R::term, lane);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < R::terms; t++) {
-                const i8 x = operand<R::fmt>(t0 + t * R::term, lane);
-#pragma unroll
-                for (int n = 0; n < TN; n++)
-                    acc[i][n] = mfma<WFMT, R::fmt>(w[n], x, acc[i][n], ws[n], xs - term_shift(t));
-            }
+            for (int n = 0; n < TN; n++)
+                acc[i][n] = mfma<WFMT, R::fmt>(w[n], x, acc[i][n], ws[n], xs[i] - term_shift(t));
+            x = next;
         }
-        __syncthreads();
+    };
+    if constexpr (DEEP) {
+        copy(j0, lds);
+        for (int j = j0; j < j1; j += 2) {
+            copy(min(j + 1, j1 - 1), lds2);
+            __builtin_amdgcn_s_waitcnt(wait_loads(COPIES));   // lds is there
+            meet();
+            multiply(lds);
+            meet();
+            if (j + 1 == j1) break;
+            copy(min(j + 2, j1 - 1), lds);
+            __builtin_amdgcn_s_waitcnt(wait_loads(COPIES));
+            meet();
+            multiply(lds2);
+            meet();
+        }
+        __builtin_amdgcn_s_waitcnt(wait_loads(0));            // no copy outlives the block
+    } else {
+        for (int j = j0; j < j1; j += PER) {
+#pragma unroll
+            for (int s = 0; s < PER; s++)
+                if (!s || j + s < j1) copy(j + s, lds + s * COPIES * NW * 1024);
+            __builtin_amdgcn_s_waitcnt(wait_loads(0));
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < PER; s++)
+                if (!s || j + s < j1) multiply(lds + s * COPIES * NW * 1024);
+            __syncthreads();
+        }
     }
 
     const int col0 = (nbw * kWTiles + wn * TN) * 16 + 4 * (lane >> 4);   // outputs col0 + 16 n + r
@@ -413,6 +461,37 @@ __global__ __launch_bounds__(128 * WM, MT == 8 || WFMT == kE3M2 ? 2 : MT == 4 ? 
             }
         }
     }
+}
+
+// Row blocks of mt tiles.  Launches of at most a block a CU take the DEEP form
+// (40 rows through 4096 x 32000 in 250 blocks 39.6 -> 32.9 us; 61 x 768 over a
+// contraction of 50304 in 255 blocks 17 us, 22 in 147 of the other form); one
+// term in 128-row blocks takes two chunks a step (2039 rows of 4 bits through
+// 4096 x 22016 130 -> 117 us).
+template <int ACT, int WFMT, int EPI>
+void gemm_launch(const Gemm& g, int mt, hipStream_t st) {
+    const dim3 grid(g.mbs * g.nbs, g.splits);
+    const bool deep = grid.x * grid.y <= 256;
+#define CGX_MX_GEMM(MT, WM, PER, DEEP) \
+    hipLaunchKernelGGL((k_gemm<ACT, WFMT, MT, WM, PER, DEEP, EPI>), grid, dim3(128 * WM), 0, st, g)
+    if (mt == 1) {
+        if (deep) CGX_MX_GEMM(1, 1, 1, true);
+        else CGX_MX_GEMM(1, 1, 1, false);
+        return;
+    }
+    if (mt == 2) {
+        if (deep) CGX_MX_GEMM(2, 2, 1, true);
+        else CGX_MX_GEMM(2, 2, 1, false);
+        return;
+    }
+    if constexpr (WFMT == kE2M1)
+        if (mt == 8) {
+            CGX_MX_GEMM(8, 2, ACT == CGX_MX_FP32 ? 1 : 2, false);
+            return;
+        }
+    if (deep) CGX_MX_GEMM(4, 4, 1, true);
+    else CGX_MX_GEMM(4, 2, 1, false);
+#undef CGX_MX_GEMM
 }
 
 // Up to 16 rows: bound by the weight's bytes.  A block takes 16 T outputs at a
@@ -600,6 +679,11 @@ __global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
         __syncthreads();                                      // the sums are read
     }
 }
+
+// Whether rows take k_gemv.  Each of its blocks cuts all of them, which costs
+// M K / 7100 us; K = 11008, 4096 outputs: one row 8.9 us, five 14.8, 16 32.4,
+// where k_gemm with its two other launches takes 20.
+inline bool gemv_pays(int M, int K) { return M <= 16 && M * (long long)K <= 80 << 10; }
 
 // Tiles a block: the fewest that leave at most a block a CU, up to eight.  One
 // block a CU and more tiles beat more blocks, each of which cuts the rows: one

@@ -84,13 +84,17 @@ struct Plan {
     int mt2, mbs2, kbs, piece;   // the second product; chunks of a piece
     size_t p, sum;
 };
+// Splits of a piece's chunks: a block a CU where few blocks would leave many
+// parts to add, two otherwise (64 rows, K = 4096, 128 chunks: 19.7 us with 16
+// splits, 20.5 with 32; 300 rows: 69 us with 3, 61 with 6).
 int splits_of(const Plan& p, int chunks) {
-    return std::max(1, std::min(512 / (p.mbs2 * p.kbs), chunks / 8));
+    const int blocks = p.mbs2 * p.kbs;
+    return std::max(1, std::min((blocks <= 64 ? 256 : 512) / blocks, chunks / 4));
 }
 Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
     Plan p = {};
     p.zt = grad ? 0 : whole((size_t)M * 4);
-    if (!grad && M <= 16) {      // k_gemv
+    if (!grad && gemv_pays(M, w->K)) {
         p.parts = gemv_groups(up(w->N, 16));
         p.part = whole((size_t)M * p.parts * sizeof(float2));
         return p;
@@ -104,7 +108,7 @@ Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
         p.part = whole((size_t)M * p.parts * sizeof(float2));
         return p;
     }
-    p.mt2 = M <= 32 ? 2 : 4;
+    p.mt2 = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     p.mbs2 = up(M, 16 * p.mt2);
     p.kbs = up(w->K, 256);
     const size_t chunk = (size_t)p.mbs2 * rows_record<CGX_MX_FP32>(p.mt2);
@@ -120,25 +124,16 @@ Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
 }
 size_t bytes(const Plan& p) { return p.rows + p.part + p.zt + p.p + p.sum; }
 
-template <int ACT, int EPI>
-void over_vocabulary(const Gemm& g, int mt) {
-    const dim3 grid(g.mbs * g.nbs);
-    if (mt == 2) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 2, 2, EPI>), grid, dim3(256), 0, stream(), g);
-    else if (mt == 4) hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 4, 2, EPI>), grid, dim3(256), 0, stream(), g);
-    else hipLaunchKernelGGL((k_gemm<ACT, kE2M1, 8, 2, EPI>), grid, dim3(256), 0, stream(), g);
-}
 template <int EPI>
 int over_vocabulary(const Gemm& g, int mt, int act) {
-    if (act == CGX_MX_FP4) over_vocabulary<CGX_MX_FP4, EPI>(g, mt);
-    else if (act == CGX_MX_FP6) over_vocabulary<CGX_MX_FP6, EPI>(g, mt);
-    else over_vocabulary<CGX_MX_FP32, EPI>(g, mt);
+    if (act == CGX_MX_FP4) gemm_launch<CGX_MX_FP4, kE2M1, EPI>(g, mt, stream());
+    else if (act == CGX_MX_FP6) gemm_launch<CGX_MX_FP6, kE2M1, EPI>(g, mt, stream());
+    else gemm_launch<CGX_MX_FP32, kE2M1, EPI>(g, mt, stream());
     return launch_check("mx loss");
 }
 template <int EPI>
 int over_inputs(const Gemm& g, int mt) {
-    const dim3 grid(g.mbs * g.nbs, g.splits);
-    if (mt == 2) hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 2, 2, EPI>), grid, dim3(256), 0, stream(), g);
-    else hipLaunchKernelGGL((k_gemm<CGX_MX_FP32, kE3M2, 4, 2, EPI>), grid, dim3(256), 0, stream(), g);
+    gemm_launch<CGX_MX_FP32, kE3M2, EPI>(g, mt, stream());
     return launch_check("mx loss gradient");
 }
 
@@ -184,7 +179,7 @@ extern "C" int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight
         float2* part = (float2*)(rows + p.rows);
         float* zt = (float*)((uint8_t*)part + p.part);
         const float* xm = x + (size_t)m0 * ld;
-        if (m <= 16) {
+        if (gemv_pays(m, w->K)) {
             Gemv g = {};
             g.x = xm;
             g.ldx = ld;
