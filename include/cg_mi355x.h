@@ -473,8 +473,8 @@ enum { CGX_MX_FP4 = 4, CGX_MX_FP6 = 6, CGX_MX_FP32 = 32 };
  * block's largest magnitude) + 125, at least 1; values are rounded to the
  * nearest, ties to even, and saturate.  A block that holds a NaN or an infinity
  * has the byte 255 and reads as NaN.  dequantize reads any byte (0: 2^-127).
- * Device pointers; rows times ceil(cols / 512) below 2^26; no output may
- * overlap another argument. */
+ * Device pointers; rows times ceil(cols / 512) below 2^26, cols at most 2^30, ld
+ * below 2^32; no output may overlap another argument. */
 int cgx_mx_quantize_dev(const float* x, size_t ld, int rows, int cols, int format,
                         uint8_t* codes, uint8_t* scales);
 int cgx_mx_dequantize_dev(const uint8_t* codes, const uint8_t* scales, int rows, int cols,
@@ -499,8 +499,8 @@ void cgx_mx_weight_free(cgx_mx_weight* w);
  * block of 32, and to 2^-130), CGX_MX_FP4 or CGX_MX_FP6 x quantised as
  * cgx_mx_quantize_dev does.  Sums are held in fp32.  A row with a NaN or an
  * infinity gets NaN, as does every row's output of a weight block of byte 255.
- * Device pointers; M below 2^23; no output or workspace may overlap another
- * argument.  ws: cgx_matmul_mx_ws bytes of device memory (16-byte aligned), for
+ * Device pointers; M below 2^23, ldx and ldy below 2^32; no output or workspace may
+ * overlap another argument.  ws: cgx_matmul_mx_ws bytes of device memory (16-byte aligned), for
  * this call alone while it runs; the size is enough for every call of at most
  * M rows with this weight and act.  Nothing is allocated: the call may be
  * captured into a graph. */

@@ -190,6 +190,22 @@ def test_rows_do_not_depend_on_each_other(gpu, act):
     assert gpu.cgx_matmul_mx_dev(w.keep[0].ptr, K, 0, w.ptr, act, w.keep[1].ptr, N, None, 0) == 0
 
 
+@pytest.mark.parametrize("M", [2, 40])
+@pytest.mark.parametrize("act", ACTS)
+def test_nan_meets_zero(gpu, M, act):
+    """A NaN of a row makes its output NaN where the weight is 0 too, and one of a weight's block where the row is 0."""
+    K, N = 128, 40
+    codes, byte, _ = R.weight(np.random.default_rng(7), N, K)
+    codes[3] = 0
+    byte[5, 2] = 255
+    w = Weight(gpu, codes, byte, K, N)
+    x = np.ones((M, K), np.float32)
+    x[0, 70] = np.nan
+    x[1] = 0
+    y = _matmul(gpu, w, x, K, N, act)
+    assert np.all(np.isnan(y[0])) and np.all(np.isnan(y[:, 5])) and np.all(np.isfinite(np.delete(y[1:], 5, 1)))
+
+
 def test_weight_bytes_of_every_size(gpu):
     """Scales 0 to 254, blocks of byte 255, and rows of small and large values."""
     rng = np.random.default_rng(6)

@@ -48,7 +48,7 @@ def test_blocks(lib, name):
         return lib.cgx_mx_dequantize_dev(codes, scales, rows, cols, fmt, x, ld)
     for kw in (dict(x=None), dict(codes=None), dict(scales=None), dict(rows=-1), dict(cols=0), dict(cols=-5), dict(ld=63), dict(ld=0),
                dict(fmt=CGX_MX_FP32), dict(fmt=0), dict(fmt=8), dict(rows=1 << 26), dict(rows=1 << 24, cols=4096, ld=4096),
-               dict(ld=1 << 32)):
+               dict(ld=1 << 32), dict(rows=1, cols=(1 << 30) + 1, ld=(1 << 30) + 1)):
         _refused(lib, call(**kw), "are required")
     for kw in (dict(codes=P + 8), dict(x=FAR + 2)):
         _refused(lib, call(**kw), "aligned")
