@@ -325,7 +325,7 @@ size_t cgk_mx_transposed_bytes(int K, int chunks);
 int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list, const int* first,
                       int chunks, uint8_t* out);
 /* records of rows, in blocks of mt tiles of 16 */
-int cgk_mx_tiles(int M, int N, int act);
+int cgk_mx_tiles(int M, int N);
 size_t cgk_mx_rows_bytes(int M, int K, int act, int mt);
 int cgk_mx_rows(const float* x, size_t ld, int M, int K, int act, int mt, uint8_t* out);
 /* y[m][n] (+)= row_scale[m] * the sum of `splits` parts, 0 in rows whose

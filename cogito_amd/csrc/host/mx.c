@@ -105,17 +105,18 @@ static int transpose(const char* who, cgx_mx_weight* w) {
     int* layers = (int*)malloc(((size_t)n * 2 + 1) * sizeof(int));
     int* dev = (int*)cgx_malloc(((size_t)n + 1) * sizeof(int));
     int rc = -1, *list = NULL;
-    if (!layers || !dev || cgx_memset(dev, 0, (size_t)n * sizeof(int)) ||
+    if (!layers) goto memory;
+    if (!dev || cgx_memset(dev, 0, (size_t)n * sizeof(int)) ||
         cgk_mx_layers(w->codes, w->K, w->N, dev) ||
         cgx_memcpy_d2h(layers, dev, (size_t)n * sizeof(int)))
         goto done;
     w->first = (int*)malloc(((size_t)n + 1) * sizeof(int));
-    if (!w->first) goto done;
+    if (!w->first) goto memory;
     w->first[0] = 0;
     for (int c = 0; c < n; c++) w->first[c + 1] = w->first[c] + (layers[c] > 1 ? layers[c] : 1);
     w->tchunks = w->first[n];
     list = (int*)malloc((size_t)w->tchunks * sizeof(int));
-    if (!list) goto done;
+    if (!list) goto memory;
     for (int c = 0; c < n; c++)
         for (int j = w->first[c]; j < w->first[c + 1]; j++) list[j] = c;
     w->list = (int*)cgx_malloc((size_t)w->tchunks * sizeof(int));
@@ -127,8 +128,10 @@ static int transpose(const char* who, cgx_mx_weight* w) {
         cgx_synchronize())
         goto done;
     rc = 0;
+    goto done;
+memory:
+    cgx_set_error("%s: out of memory", who);
 done:
-    if (rc && !*cgx_last_error()) cgx_set_error("%s: out of memory", who);
     free(layers);
     free(list);
     cgx_free(dev);

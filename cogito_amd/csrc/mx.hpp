@@ -204,9 +204,10 @@ typedef const __attribute__((address_space(4))) int* constant_ints;   // read by
 // s_waitcnt's operand that waits until n of a wave's loads are outstanding
 constexpr int wait_loads(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
 
-// The block's waves meet; what the compiler moves over no side of it.
+// The block's waves meet, their reads of LDS done; the compiler moves none over it.
 __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);                       // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }

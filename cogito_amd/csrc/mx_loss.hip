@@ -99,7 +99,7 @@ Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
         p.part = whole((size_t)M * p.parts * sizeof(float2));
         return p;
     }
-    p.mt = cgk_mx_tiles(M, w->N, act);
+    p.mt = cgk_mx_tiles(M, w->N);
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
     p.parts = 2 * p.nbs;
