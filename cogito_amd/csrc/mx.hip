@@ -436,9 +436,7 @@ Plan plan(const cgx_mx_weight* w, int M, int act) {
     p.mt = cgk_mx_tiles(M, w->N);
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
-    const int kc = up(w->K, 128), blocks = p.mbs * p.nbs;
-    // a join costs what four or five chunks of a block do
-    p.splits = std::max(1, std::min(512 / blocks, kc < 16 ? 1 : kc / 4));
+    p.splits = gemm_splits(p.mbs * p.nbs, up(w->K, 128));
     p.rows = (cgk_mx_rows_bytes(M, w->K, act, p.mt) + 255) & ~(size_t)255;
     p.part = p.splits > 1 ? (size_t)p.splits * M * ((w->N + 3) & ~3) * 4 : 0;
     return p;

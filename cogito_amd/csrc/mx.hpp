@@ -509,6 +509,14 @@ void gemm_launch(const Gemm& g, int mt, hipStream_t st) {
 #undef CGX_MX_GEMM
 }
 
+// Splits of a contraction of kc chunks over which `blocks` blocks go: two blocks a
+// CU, of at least four chunks each (a join costs what four or five chunks of a
+// block do).
+inline int gemm_splits(int blocks, int kc) {
+    const int s = 512 / blocks, most = kc < 16 ? 1 : kc / 4;
+    return s < 1 ? 1 : s < most ? s : most;
+}
+
 // Up to 16 rows: bound by the weight's bytes.  A block takes 16 T outputs at a
 // time and its waves the chunks of the contraction in turn, operands of the
 // weight going from memory to registers D chunks ahead.  The block cuts the

@@ -509,7 +509,7 @@ int cgx_matmul_mx_dev(const float* x, size_t ldx, int M, const cgx_mx_weight* w,
                       float* y, size_t ldy, void* ws, size_t ws_bytes);
 
 /* Softmax cross entropy over the vocabulary of an lm_head W [K][V], from hidden
- * rows h [rows][K] (ldh floats apart), without storing a logit: with
+ * rows h [rows][K] (ldh floats apart), keeping no logits: with
  * z = h' W (h' as in cgx_matmul_mx_dev), lse[m] = log sum exp z[m] and
  * loss[m] = lse[m] - z[m][targets[m]], 0 for a target outside [0, V) (an
  * ignored row).  loss or lse may be NULL.  A row with a logit that is NaN or
