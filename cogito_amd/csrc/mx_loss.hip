@@ -2,7 +2,7 @@
 // lm_head, from hidden rows, and its gradient with respect to them.
 //
 // With z = x W: lse = log sum exp z, loss = lse - z[target].  The product's
-// epilogue leaves a maximum, a sum and the target's logit for each row and
+// epilogue leaves a sum over the largest and the target's logit for each row and
 // 128 outputs; a second launch joins a row's.
 //
 // Gradient: dx = g ((p - e_target) W^T), p = exp(z - lse).  Over pieces of the
@@ -42,10 +42,9 @@ struct Sum {
     double sum;
 };
 __device__ __forceinline__ Sum join(Sum a, Sum b) {
-    // a part without a value above -inf holds 0, or NaN
-    const float top = fmaxf(a.top, b.top), ref = top == -INFINITY ? 0.0f : top;
-    const float ea = a.top == -INFINITY ? 1.0f : expf(a.top - ref);
-    const float eb = b.top == -INFINITY ? 1.0f : expf(b.top - ref);
+    const float top = fmaxf(a.top, b.top), ref = over(top);
+    const float ea = a.top == -INFINITY ? 1.0f : exp_over(a.top, ref);
+    const float eb = b.top == -INFINITY ? 1.0f : exp_over(b.top, ref);
     return {top, a.sum * ea + b.sum * eb};
 }
 __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, int parts,
@@ -71,7 +70,7 @@ __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, i
     if (threadIdx.x) return;
 #pragma unroll
     for (int w = 1; w < 4; w++) s = join(s, wave[w]);
-    const double l = (double)(s.top == -INFINITY ? 0.0f : s.top) + log(s.sum);
+    const double l = (double)over(s.top) + log(s.sum);
     const int t = targets[m];
     if (lse) lse[m] = (float)l;
     if (loss) loss[m] = t >= 0 && t < V ? (float)(l - (double)zt[m]) : 0.0f;
@@ -91,7 +90,7 @@ __device__ __forceinline__ f4 sum_of(const float* p, int splits, size_t stride, 
     return v;
 }
 
-// The epilogue's maximum and sum, a block 1024 outputs of a row.
+// The epilogue's parts, a block 1024 outputs of a row.
 __global__ __launch_bounds__(256) void k_stats(const float* __restrict__ z, int splits, size_t stride,
                                                int pld, int N, const int* __restrict__ targets,
                                                float2* __restrict__ part, float* __restrict__ zt) {
@@ -111,9 +110,9 @@ __global__ __launch_bounds__(256) void k_stats(const float* __restrict__ z, int 
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float ref = top == -INFINITY ? 0.0f : top;
+    const float ref = over(top);
 #pragma unroll
-    for (int r = 0; r < 4; r++) sum += expf(v[r] - ref);
+    for (int r = 0; r < 4; r++) sum += exp_over(v[r], ref);
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) wave[threadIdx.x >> 6] = make_float2(top, sum);
@@ -145,7 +144,7 @@ __global__ __launch_bounds__(256) void k_probs(const float* __restrict__ z, int 
         if (live && n < N) q = sum_of(z + (size_t)m * pld, splits, stride, n);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            float p = live && n + r < N ? expf(q[r] - l) : 0.0f;
+            float p = live && n + r < N ? exp_over(q[r], l) : 0.0f;
             if (live && n + r == t) p = expm1f(q[r] - l);
             set(v, 4 * i + r, p);
         }

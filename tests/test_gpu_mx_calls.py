@@ -195,3 +195,29 @@ def test_quantised_rows_are_what_the_product_takes(gpu):
         _ok(gpu, gpu.cgx_mx_quantize_dev(d.ptr, K, n, K, fmt, c.ptr, s.ptr) or
             gpu.cgx_mx_dequantize_dev(c.ptr, s.ptr, n, K, fmt, back.ptr, K))
         np.testing.assert_array_equal(_matmul(gpu, w, back.numpy(np.float32, (n, K)), K, N, fmt), _matmul(gpu, w, x, K, N, fmt))
+
+
+@pytest.mark.parametrize("rows,K", [(3, 32), (20, 32), (20, 4096)])
+def test_logits_at_the_ends_of_the_range(gpu, rows, K):
+    """Logits up to 3 2^126, exact: no difference of theirs leaves the range unnoticed."""
+    V = 300
+    w = np.zeros((V, K), np.float32)
+    w[:, 0] = 0.5
+    w[7, 0], w[9, 1], w[:, 2], w[11, 3] = 2, 3, -3, -3
+    c, b = R.quantise(w, 4)
+    h = np.zeros((rows, K), np.float32)
+    big = np.float32(2.0 ** 126)
+    h[0, 0] = h[1, 1] = h[2, 2] = big
+    if rows > 3:
+        h[3, 3] = big
+        h[5, 0], h[6, 0] = 2.0 ** 40, 2.0 ** 24
+    t = np.full(rows, 7, np.int32)
+    loss, lse, dh = Loss(gpu, Weight(gpu, R.pack(c, 4), b, K, V, grad=1), h, t, CGX_MX_FP32, V).run()
+    assert lse[0] == 2 * big and loss[0] == 0 and np.all(dh[0] == 0)
+    assert lse[1] == 3 * big and loss[1] == 3 * big and dh[1, 1] == 3 and dh[1, 0] == 0.5 - 2
+    assert lse[2] == -3 * big
+    if rows > 3:
+        # one token of no mass, 299 alike: off by the fp32 sums of 300 terms and lse's rounding
+        assert abs(lse[3] - np.log(299.0)) < 2.0 ** -15 and abs(loss[3] - np.log(299.0)) < 2.0 ** -15
+        assert abs(lse[4] - np.log(300.0)) < 2.0 ** -15
+        assert lse[5] == 2.0 ** 41 and lse[6] == 2.0 ** 25 and not loss[5:7].any() and not dh[5:7].any()
