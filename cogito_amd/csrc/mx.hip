@@ -274,7 +274,8 @@ __global__ __launch_bounds__(256) void k_rows(const float* __restrict__ x, size_
     // rows past the last repeat it: nothing of theirs is stored
     const int m = min(tile * 16 + (lane & 15), M - 1);
     Block v;
-    load_block(v, x + (size_t)m * ld, c * 128 + (lane >> 4) * 32, K, c * 128 + 128 <= K);
+    const int k = c * 128 + (lane >> 4) * 32;
+    load_block(v, x + (size_t)m * ld, k, K, k + 32 <= K);
     using R = Rows<ACT>;
     const int b = tile / mt, at = tile - b * mt;
     uint8_t* rec = out + ((size_t)b * kc + c) * (size_t)rows_record<ACT>(mt);

@@ -151,9 +151,10 @@ __device__ __forceinline__ void put(uint8_t* tile, uint8_t* sc, int lane, Block&
     });
 }
 
-// The block from value k of a row on, 0 past the row's end.  whole: every
-// lane's block lies within its row; the loads go to where the conversion reads,
-// so that they stay in flight until then.
+// The block from value k of a row on, 0 past the row's end.  whole: the lane's
+// block lies within the row; the loads go to where the conversion reads, so that
+// they stay in flight until then.  (Value by value in every lane, rows that end
+// inside a block took 16.5 us for 12 x 2229 through 6144 outputs, now 9.1.)
 __device__ __forceinline__ void load_block(Block& b, const float* x, int k, int cols, bool whole) {
     if (whole) {
 #pragma unroll
@@ -609,14 +610,14 @@ __global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
         for (int t = 0; t < T; t++) acc[t] = f4{0, 0, 0, 0};
         for (int c0 = 0; c0 < a.kc; c0 += a.seg) {
             const int n = min(a.seg, a.kc - c0), blocks = 4 * n, total = a.M * blocks;
-            const bool whole = c0 * 128 + blocks * 32 <= a.K;
             if (c0) __syncthreads();                          // the last segment is multiplied
             if (fresh)
                 for (int u0 = wave * 64; u0 < total; u0 += 64 * kGemvWaves) {
                     // lanes past the end repeat the last block
                     const int u = min(u0 + lane, total - 1), m = u / blocks, b = u - m * blocks;
                     Block x;
-                    load_block(x, a.x + (size_t)m * a.ldx, c0 * 128 + b * 32, a.K, whole);
+                    const int k = c0 * 128 + b * 32;
+                    load_block(x, a.x + (size_t)m * a.ldx, k, a.K, k + 32 <= a.K);
                     const int top = cut<ACT>(x, [&](int t, i8 v) {
                         const int at = (t * a.M + m) * ld + b;
                         *(i4*)(lds + at * 16) = i4{v[0], v[1], v[2], v[3]};
