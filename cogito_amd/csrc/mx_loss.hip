@@ -100,11 +100,11 @@ __global__ __launch_bounds__(256) void k_stats(const float* __restrict__ z, int 
     float top = -INFINITY, sum = 0.0f;
     if (n < N) {
         v = sum_of(z + (size_t)m * pld, splits, stride, n);
-        const int t = targets[m] - n;
+        const int t = targets[m];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             v[r] = n + r < N ? v[r] : -INFINITY;
-            if (t == r && n + r < N) zt[m] = v[r];
+            if (n + r == t && t < N) zt[m] = v[r];
             top = fmaxf(top, v[r]);
         }
     }
