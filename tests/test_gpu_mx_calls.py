@@ -221,3 +221,38 @@ def test_logits_at_the_ends_of_the_range(gpu, rows, K):
         assert abs(lse[3] - np.log(299.0)) < 2.0 ** -15 and abs(loss[3] - np.log(299.0)) < 2.0 ** -15
         assert abs(lse[4] - np.log(300.0)) < 2.0 ** -15
         assert lse[5] == 2.0 ** 41 and lse[6] == 2.0 ** 25 and not loss[5:7].any() and not dh[5:7].any()
+
+
+@pytest.mark.parametrize("act", [CGX_MX_FP4, CGX_MX_FP6, CGX_MX_FP32])
+@pytest.mark.parametrize("M,K,N,ld", [(12, 2229, 600, 2230), (1, 3611, 100, 3611), (7, 10001, 90, 10003), (16, 31, 70, 40), (3, 97, 4100, 98), (16, 5089, 33, 5100)])
+def test_few_rows_that_end_inside_a_block(gpu, M, K, N, ld, act):
+    """NaN behind every row; rows at any alignment; over one segment of the contraction and several."""
+    rng = np.random.default_rng(M * K + N)
+    codes, byte, W = R.weight(rng, N, K, 0.1, 2)
+    x = _rows(rng, M, K)
+    y = _matmul(gpu, Weight(gpu, codes, byte, K, N), x, K, N, act, ldx=ld, ldy=N + 1, offx=1, offy=3)
+    xt = R.taken(x, act)
+    _within(y - xt @ W, _tol(np.abs(xt), R.cut_error(x, act), W, K, act))
+
+
+def test_blocks_captured(gpu):
+    """Quantisation and read-back replayed over other values at the same addresses."""
+    rng = np.random.default_rng(36)
+    n, K = 37, 1000
+    d, c, s, back = (DeviceArray(gpu, b) for b in (n * K * 4, n * 32 * 24, n * 32, n * K * 4))
+    for fmt in (CGX_MX_FP4, CGX_MX_FP6):
+        d.upload(_rows(rng, n, K))
+        assert gpu.cgx_graph_begin() == 0
+        rc = gpu.cgx_mx_quantize_dev(d.ptr, K, n, K, fmt, c.ptr, s.ptr) or gpu.cgx_mx_dequantize_dev(c.ptr, s.ptr, n, K, fmt, back.ptr, K)
+        graph = gpu.cgx_graph_end()
+        assert rc == 0 and graph, last_error(gpu)
+        for _ in range(3):
+            x = _rows(rng, n, K)
+            d.upload(x)
+            assert gpu.cgx_graph_launch(graph) == 0
+            _ok(gpu, 0)
+            got = back.numpy(np.float32, (n, K)).copy()
+            np.testing.assert_array_equal(got, R.taken(x, fmt).astype(np.float32))
+            _ok(gpu, gpu.cgx_mx_quantize_dev(d.ptr, K, n, K, fmt, c.ptr, s.ptr) or gpu.cgx_mx_dequantize_dev(c.ptr, s.ptr, n, K, fmt, back.ptr, K))
+            np.testing.assert_array_equal(back.numpy(np.float32, (n, K)), got)
+        assert gpu.cgx_graph_free(graph) == 0
