@@ -433,7 +433,7 @@ struct Plan {
 };
 Plan plan(const cgx_mx_weight* w, int M, int act) {
     Plan p = {};
-    if (gemv_pays(M, w->K)) return p;
+    if (gemv_pays(M, w->K, w->N)) return p;
     p.mt = cgk_mx_tiles(M, w->N);
     p.mbs = up(M, 16 * p.mt);
     p.nbs = up(w->N, 256);
@@ -491,7 +491,7 @@ extern "C" int cgk_mx_matmul(const float* x, size_t ldx, int M, const cgx_mx_wei
         const Plan p = plan(w, m, act);
         const float* xm = x + (size_t)m0 * ldx;
         float* ym = y + (size_t)m0 * ldy;
-        if (gemv_pays(m, w->K)) {
+        if (gemv_pays(m, w->K, w->N)) {
             Gemv g = {};
             g.x = xm;
             g.ldx = ldx;

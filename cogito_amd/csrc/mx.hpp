@@ -714,9 +714,15 @@ __global__ __launch_bounds__(64 * kGemvWaves) void k_gemv(const Gemv a) {
 }
 
 // Whether rows take k_gemv.  Each of its blocks cuts all of them, which costs
-// M K / 7100 us; K = 11008, 4096 outputs: one row 8.9 us, five 14.8, 16 32.4,
-// where k_gemm with its two other launches takes 20.
-inline bool gemv_pays(int M, int K) { return M <= 16 && M * (long long)K <= 80 << 10; }
+// M K / 7100 us, against k_gemm's launch or two besides: 4096 outputs, K = 4096, ten
+// rows 10.8 us, with k_gemm 11.8, twelve 11.5 and 11.8; K = 10208, three 12.3 and 13.7,
+// eight 20.5 and 14.1.  From 256 blocks of 256 outputs on k_gemm fills the card
+// with any rows: 128256 outputs with their loss, one row of K = 768 22.5 and 17.1, of
+// 4096 55.3 and 56.5, ten 84.0 and 56.1 (50257: one of 768 13.8 and 13.6, of 4096 28.8
+// and 33.9).
+inline bool gemv_pays(int M, int K, int N) {
+    return M <= 16 && M * (long long)K <= 48 << 10 && N <= 65536;
+}
 
 // Tiles a block: the fewest that leave at most a block a CU, up to eight.  One
 // block a CU and more tiles beat more blocks, each of which cuts the rows: one

@@ -177,7 +177,7 @@ Plan plan(const cgx_mx_weight* w, int M, int act, int grad) {
     Plan p = {};
     const int kc = up(w->K, 128), pld = (w->N + 3) & ~3;
     p.zt = grad ? 0 : whole((size_t)M * 4);
-    if (!grad && gemv_pays(M, w->K)) {
+    if (!grad && gemv_pays(M, w->K, w->N)) {
         p.parts = gemv_groups(up(w->N, 16));
         p.part = whole((size_t)M * p.parts * sizeof(float2));
         return p;
@@ -278,7 +278,7 @@ extern "C" int cgk_mx_loss(const float* x, size_t ld, int M, const cgx_mx_weight
         float* zt = (float*)((uint8_t*)part + p.part);
         float* z = (float*)((uint8_t*)zt + p.zt);
         const float* xm = x + (size_t)m0 * ld;
-        if (gemv_pays(m, w->K)) {
+        if (gemv_pays(m, w->K, w->N)) {
             Gemv g = {};
             g.x = xm;
             g.ldx = ld;
