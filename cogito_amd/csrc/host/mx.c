@@ -13,8 +13,8 @@
 #include "cgx_internal.h"
 
 /* MAX_ROWS as in paged.c; MAX_WAVES: a wave a row's 512 values, four a block of
- * 256 threads, within a launch's 2^32 threads */
-enum { MAX_ROWS = 1 << 23, MAX_K = 1 << 20, MAX_N = 1 << 24, MAX_WAVES = 1 << 26,
+ * 256 threads: 2^24 - 1 blocks, as a launch has fewer than 2^32 threads */
+enum { MAX_ROWS = 1 << 23, MAX_K = 1 << 20, MAX_N = 1 << 24, MAX_WAVES = (1 << 26) - 4,
        MAX_COLS = 1 << 30 };
 
 static int misaligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
@@ -28,11 +28,11 @@ static int check_format(const char* who, const float* x, size_t ld, int rows, in
                         const uint8_t* codes, const uint8_t* scales) {
     if (!x || !codes || !scales || rows < 0 || cols < 1 || cols > MAX_COLS ||
         ld < (size_t)cols ||
-        ld >= (size_t)1 << 32 || (long long)rows * ((cols + 511LL) / 512) >= MAX_WAVES ||
+        ld >= (size_t)1 << 32 || (long long)rows * ((cols + 511LL) / 512) > MAX_WAVES ||
         (format != CGX_MX_FP4 && format != CGX_MX_FP6)) {
         cgx_set_error("%s: rows of cols >= 1 values, ld >= cols apart, to or from CGX_MX_FP4 or "
                       "CGX_MX_FP6 codes and scales are required (rows times ceil(cols / 512) "
-                      "below 2^26, cols at most 2^30, ld below 2^32)", who);
+                      "at most 2^26 - 4, cols at most 2^30, ld below 2^32)", who);
         return -1;
     }
     if (misaligned(codes, 16) || misaligned(x, 4)) {

@@ -473,8 +473,8 @@ enum { CGX_MX_FP4 = 4, CGX_MX_FP6 = 6, CGX_MX_FP32 = 32 };
  * block's largest magnitude) + 125, at least 1; values are rounded to the
  * nearest, ties to even, and saturate.  A block that holds a NaN or an infinity
  * has the byte 255 and reads as NaN.  dequantize reads any byte (0: 2^-127).
- * Device pointers; rows times ceil(cols / 512) below 2^26, cols at most 2^30, ld
- * below 2^32; no output may overlap another argument. */
+ * Device pointers; rows times ceil(cols / 512) at most 2^26 - 4, cols at most 2^30,
+ * ld below 2^32; no output may overlap another argument. */
 int cgx_mx_quantize_dev(const float* x, size_t ld, int rows, int cols, int format,
                         uint8_t* codes, uint8_t* scales);
 int cgx_mx_dequantize_dev(const uint8_t* codes, const uint8_t* scales, int rows, int cols,
