@@ -303,13 +303,14 @@ int cgk_logprobs(const float* x, size_t ld, int rows, int V, const int* tokens, 
 /* Microscaled weights (mx.hip, mx_loss.hip); arguments checked by host/mx.c.
  * A weight is records of 256 outputs and 128 inputs; with a gradient also its
  * transpose, records of 256 inputs and a chunk of 128 outputs, first[c] ..
- * first[c + 1] - 1 those of chunk c (list: the chunk of each). */
+ * first[c + 1] - 1 those of chunk c, one a layer of it that holds values (list: the
+ * chunk of each, then the layer of each). */
 struct cgx_mx_weight {
     int K, N;
     uint8_t* codes;
     int chunks128;           /* chunks of 128 outputs */
     uint8_t* tcodes;         /* NULL: no gradient */
-    int* list;               /* device, [tchunks] */
+    int* list;               /* device, [2][tchunks] */
     int* first;              /* host, [chunks128 + 1] */
     int tchunks;
 };
@@ -320,9 +321,9 @@ int cgk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int rows, int
 size_t cgk_mx_weight_bytes(int K, int N);
 int cgk_mx_weight(const uint8_t* codes, const uint8_t* scales, int K, int N, uint8_t* w);
 int cgk_mx_weight_of(const float* x, int K, int N, uint8_t* w);
-int cgk_mx_layers(const uint8_t* w, int K, int N, int* layers);
+int cgk_mx_layers(const uint8_t* w, int K, int N, uint64_t* layers);   /* a bit each */
 size_t cgk_mx_transposed_bytes(int K, int chunks);
-int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list, const int* first,
+int cgk_mx_transposed(const uint8_t* w, int K, int N, const int* list, const int* layers,
                       int chunks, uint8_t* out);
 /* records of rows, in blocks of mt tiles of 16 */
 int cgk_mx_tiles(int M, int N);

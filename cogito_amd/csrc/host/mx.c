@@ -98,33 +98,36 @@ static cgx_mx_weight* weight(const char* who, int K, int N) {
     return w;
 }
 
-/* The transposed copy: layers of every chunk counted on the device, the list
- * of chunks made here. */
+/* The transposed copy: the layers of every chunk found on the device, the list of
+ * chunks and layers made here.  Layer 0 is always there. */
 static int transpose(const char* who, cgx_mx_weight* w) {
     const int n = w->chunks128;
-    int* layers = (int*)malloc(((size_t)n * 2 + 1) * sizeof(int));
-    int* dev = (int*)cgx_malloc(((size_t)n + 1) * sizeof(int));
+    uint64_t* layers = (uint64_t*)malloc((size_t)n * sizeof(uint64_t));
+    uint64_t* dev = (uint64_t*)cgx_malloc((size_t)n * sizeof(uint64_t));
     int rc = -1, *list = NULL;
     if (!layers) goto memory;
-    if (!dev || cgx_memset(dev, 0, (size_t)n * sizeof(int)) ||
+    if (!dev || cgx_memset(dev, 0, (size_t)n * sizeof(uint64_t)) ||
         cgk_mx_layers(w->codes, w->K, w->N, dev) ||
-        cgx_memcpy_d2h(layers, dev, (size_t)n * sizeof(int)))
+        cgx_memcpy_d2h(layers, dev, (size_t)n * sizeof(uint64_t)))
         goto done;
     w->first = (int*)malloc(((size_t)n + 1) * sizeof(int));
     if (!w->first) goto memory;
     w->first[0] = 0;
-    for (int c = 0; c < n; c++) w->first[c + 1] = w->first[c] + (layers[c] > 1 ? layers[c] : 1);
+    for (int c = 0; c < n; c++) w->first[c + 1] = w->first[c] + __builtin_popcountll(layers[c] | 1);
     w->tchunks = w->first[n];
-    list = (int*)malloc((size_t)w->tchunks * sizeof(int));
+    list = (int*)malloc((size_t)w->tchunks * 2 * sizeof(int));
     if (!list) goto memory;
-    for (int c = 0; c < n; c++)
-        for (int j = w->first[c]; j < w->first[c + 1]; j++) list[j] = c;
-    w->list = (int*)cgx_malloc((size_t)w->tchunks * sizeof(int));
+    for (int c = 0, j = 0; c < n; c++)
+        for (uint64_t left = layers[c] | 1; left; left &= left - 1, j++) {
+            list[j] = c;
+            list[w->tchunks + j] = __builtin_ctzll(left);
+        }
+    w->list = (int*)cgx_malloc((size_t)w->tchunks * 2 * sizeof(int));
     w->tcodes = (uint8_t*)cgx_malloc(cgk_mx_transposed_bytes(w->K, w->tchunks));
     if (!w->list || !w->tcodes ||
-        cgx_memcpy_h2d(w->list, list, (size_t)w->tchunks * sizeof(int)) ||
-        cgx_memcpy_h2d(dev, w->first, (size_t)n * sizeof(int)) ||
-        cgk_mx_transposed(w->codes, w->K, w->N, w->list, dev, w->tchunks, w->tcodes) ||
+        cgx_memcpy_h2d(w->list, list, (size_t)w->tchunks * 2 * sizeof(int)) ||
+        cgk_mx_transposed(w->codes, w->K, w->N, w->list, w->list + w->tchunks, w->tchunks,
+                          w->tcodes) ||
         cgx_synchronize())
         goto done;
     rc = 0;

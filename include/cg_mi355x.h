@@ -485,8 +485,11 @@ int cgx_mx_dequantize_dev(const uint8_t* codes, const uint8_t* scales, int rows,
  * and scales [N][ceil(K / 32)] as cgx_mx_quantize_dev writes them, host or
  * device; cgx_mx_weight_from_tensor quantises W, [K, N] as in cg_quantize_int4,
  * host or device, in blocks along K.  grad: 1 for a weight that
- * cgx_token_loss_mx_grad_dev takes, which keeps a transposed copy as well
- * (25/32 bytes a value).  K at most 2^20, N at most 2^24, K N at most 2^36.
+ * cgx_token_loss_mx_grad_dev takes, which keeps a transposed copy as well: 25/32
+ * bytes a value where the scales of 32 neighbouring outputs lie within six powers of
+ * two of each other in every input; 128 outputs hold all their inputs once more for
+ * each further range of six that such a block of theirs has values in (at most
+ * 43 times, and the gradient's second product grows alike).  K at most 2^20, N at most 2^24, K N at most 2^36.
  * NULL on an error. */
 typedef struct cgx_mx_weight cgx_mx_weight;
 cgx_mx_weight* cgx_mx_weight_new(const uint8_t* codes, const uint8_t* scales, int K, int N,
