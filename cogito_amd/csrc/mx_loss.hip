@@ -122,17 +122,17 @@ __global__ __launch_bounds__(256) void k_stats(const float* __restrict__ z, int 
     part[((size_t)m * gridDim.x + blockIdx.x) * 4 + threadIdx.x] = wave[threadIdx.x];
 }
 
-// The epilogue's p - e_target as records: a wave a tile of 16 rows and a chunk,
-// a lane a block of 32 outputs.
+// The epilogue's p - e_target as records of a piece from chunk c0 of the vocabulary
+// on: a wave a tile of 16 rows and a chunk, a lane a block of 32 outputs.
 __global__ __launch_bounds__(256) void k_probs(const float* __restrict__ z, int splits, size_t stride,
                                                int pld, int M, int N, const int* __restrict__ targets,
-                                               const float* __restrict__ lse, int chunks, int mt,
-                                               int units, uint8_t* __restrict__ out) {
+                                               const float* __restrict__ lse, int c0, int chunks,
+                                               int mt, int units, uint8_t* __restrict__ out) {
     const int u = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (u >= units) return;
     const int lane = threadIdx.x & 63, tile = u / chunks, c = u - tile * chunks;
     // rows past the last repeat it: nothing of theirs is stored
-    const int m = min(tile * 16 + (lane & 15), M - 1), n0 = c * 128 + (lane >> 4) * 32;
+    const int m = min(tile * 16 + (lane & 15), M - 1), n0 = (c0 + c) * 128 + (lane >> 4) * 32;
     const int t = targets[m];
     const bool live = t >= 0 && t < N;
     const float l = live ? lse[m] : 0.0f;
@@ -334,11 +334,10 @@ extern "C" int cgk_mx_loss_grad(const float* x, size_t ld, int M, const cgx_mx_w
             g.nb0 = c / 2;
             g.nbs = up(e - c, 2);
             if (p.splits > 1) {
-                // so few blocks are one piece: at most 170 of 64 rows and 256 outputs
                 if (split_logits(g, p.mt, act, z)) return -1;
                 const int units = p.mbs2 * p.mt2 * p.piece;
                 hipLaunchKernelGGL(k_probs, dim3(up(units, 4)), dim3(256), 0, stream(), z, p.splits,
-                                   g.stride, (int)g.ld, m, w->N, targets + m0, lse + m0, p.piece,
+                                   g.stride, (int)g.ld, m, w->N, targets + m0, lse + m0, c, p.piece,
                                    p.mt2, units, probs);
                 if (launch_check("mx loss probabilities")) return -1;
             } else {
