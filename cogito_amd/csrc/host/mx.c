@@ -232,6 +232,15 @@ static int check_ld(const char* who, const float* x, size_t ld, int cols) {
     return 0;
 }
 
+/* a loss's arrays of a value a row; optional ones are NULL */
+static int check_arrays(const char* who, const int* targets, const float* a, const float* b) {
+    if (misaligned(targets, 4) || misaligned(a, 4) || misaligned(b, 4)) {
+        cgx_set_error("%s: targets and the values of a row have to be 4-byte aligned", who);
+        return -1;
+    }
+    return 0;
+}
+
 size_t cgx_matmul_mx_ws(const cgx_mx_weight* w, int M, int act) {
     if (check_rows("cgx_matmul_mx_ws", w, M, act)) return 0;
     return cgk_mx_matmul_ws(w, M, act);
@@ -280,6 +289,7 @@ int cgx_token_loss_mx_dev(const float* h, size_t ldh, int rows, const cgx_mx_wei
         cgx_set_error("%s: targets and loss or lse are required", who);
         return -1;
     }
+    if (check_arrays(who, targets, loss, lse)) return -1;
     const size_t need = cgk_mx_loss_need(w, rows, act, 0), T = (size_t)rows;
     if (check_ws(who, ws, ws_bytes, need)) return -1;
     const cgx_span mem[] = {{loss, T * 4, 1},
@@ -304,6 +314,7 @@ int cgx_token_loss_mx_grad_dev(const float* h, size_t ldh, int rows, const cgx_m
         cgx_set_error("%s: targets and lse are required", who);
         return -1;
     }
+    if (check_arrays(who, targets, lse, dloss)) return -1;
     const size_t need = cgk_mx_loss_need(w, rows, act, 1), T = (size_t)rows;
     if (check_ws(who, ws, ws_bytes, need)) return -1;
     const cgx_span mem[] = {{dh, row_bytes(rows, ldd, w->K), 1},

@@ -522,7 +522,8 @@ int cgx_matmul_mx_dev(const float* x, size_t ldx, int M, const cgx_mx_weight* w,
  * [rows] the gradient of each row's loss (NULL: 1), and 0 for an ignored row;
  * a quantised h' passes its gradient on to h.  dh is written, not added to.
  * ws: cgx_token_loss_mx_ws bytes (grad: 1 for the gradient, whose size is
- * enough for both calls), as in cgx_matmul_mx_dev, which says the rest. */
+ * enough for both calls), as in cgx_matmul_mx_dev, which says the rest; targets,
+ * loss, lse and dloss are 4-byte aligned. */
 size_t cgx_token_loss_mx_ws(const cgx_mx_weight* w, int rows, int act, int grad);
 int cgx_token_loss_mx_dev(const float* h, size_t ldh, int rows, const cgx_mx_weight* w, int act,
                           const int* targets, float* loss, float* lse, void* ws,
