@@ -461,9 +461,11 @@ void gemv(const Gemv& g) {
 }  // namespace
 
 // Tiles of a row block: 128 rows unless 64 leave a tenth fewer rows empty (fp32
-// rows through 4096 x 32000: 1024 rows 304 us, with 64-row blocks 338; 301 rows
-// through 4096 x 128256: 447 us, 412), half where that leaves a CU without two blocks
-// (61 rows through 768 x 50257: 13.6 us with 32 rows, 15.4 with 64).
+// rows: 1024 through 4096 x 32000 304 us, with 64-row blocks 314, with 32-row ones 355;
+// the loss of 301 over 4096 x 128256 374 us with 64, 438 with 128, 408 with 32), half
+// where that leaves a CU without two blocks (200 through 4096 x 4096: 23 us with 32
+// rows, 26 with 64, 31 with 128; 64: 14.9, 16.6 and 23.9; 61 through 768 x 50257: 16.2,
+// 16.7 and 28.7, where one term prefers 64: 11.9 and 11.3).
 extern "C" int cgk_mx_tiles(int M, int N) {
     if (M <= 16) return 1;
     int mt = 10 * up(M, 128) * 128 <= 11 * up(M, 64) * 64 ? 8 : 4;

@@ -9,9 +9,13 @@
 // with an 8-bit one, so nothing here is held in 8 bits.  Rates, measured with
 // operands in registers: 7.4-7.6 PFLOP/s 4 x 4 bits, 6.3 6 x 4, 6.8-7.1 6 x 6.
 //
-// Rows taken as they are (CGX_MX_FP32) are five 6-bit (E2M3) terms of the same
+// Rows that are not quantised (CGX_MX_FP32) are five 6-bit (E2M3) terms of the same
 // block: each term rounds what the ones before left, 5 bits a term, so that a
-// value is held to 2^-23 of the largest of its block.  With 6.3 / 5 = 1.26
+// value is held to 2^-23 of the largest of its block (32/31 2^-24 by the terms' own
+// steps), as fp32 holds that largest one.  The block's others are held to less than
+// fp32 holds them, by their distance from it: an outlier channel a thousand times its
+// neighbours leaves them 14 bits, which an output sees where the outlier's own weight
+// is near 0 (elsewhere an fp32 sum would round as much).  With 6.3 / 5 = 1.26
 // PFLOP/s of the product this beats two fp16 halves (0.70 at the rate measured for them),
 // and the weight needs no decoding.
 #pragma once
@@ -246,7 +250,7 @@ enum { kStore = 0, kGrad = 1, kStats = 2, kProbs = 3 };
 // e^(z - z0), z0 not below z by much: the hardware's 2^x (an ulp) of the difference
 // times log2(e).  Its two roundings cost 2^-24 |z - z0| of the result, which is the
 // smaller the larger that is.  301 rows over 4096 x 128256 364 us, with expf 371; 1184
-// rows over 37 x 32000 28, 39.
+// quantised rows over 37 x 32000 28, 39.
 __device__ __forceinline__ float exp_over(float z, float z0) {
     return __builtin_amdgcn_exp2f((z - z0) * 1.44269504f);
 }
@@ -724,7 +728,9 @@ inline bool gemv_pays(int M, int K, int N) {
     return M <= 16 && M * (long long)K <= 48 << 10 && N <= 65536;
 }
 
-// Tiles a block: the fewest that leave at most a block a CU, up to eight.  One
+// Tiles a block: the fewest of 1, 2, 3, 4, 6 and 8 (each a kernel of its own for every
+// kind of rows and epilogue: 5 and 7 are left out, for whose outputs 171 to 224 blocks
+// of 6 or 8 tiles stand) that leave at most a block a CU, up to eight.  One
 // block a CU and more tiles beat more blocks, each of which cuts the rows: one
 // row through 4096 x 22016 10.3 us with 6 tiles (230 blocks), 13.2 with 3.
 inline int gemv_tiles(int tiles) {

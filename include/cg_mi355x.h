@@ -498,8 +498,10 @@ cgx_mx_weight* cgx_mx_weight_from_tensor(cg_tensor* W, int grad);
 void cgx_mx_weight_free(cgx_mx_weight* w);
 
 /* y [M][N] = x' W, x [M][K] rows of floats (ldx and ldy apart).  act says what
- * x' is: CGX_MX_FP32 x itself (each value held to 2^-23 of the largest of its
- * block of 32, and to 2^-130), CGX_MX_FP4 or CGX_MX_FP6 x quantised as
+ * x' is: CGX_MX_FP32 x with each value held to 2^-23 of the largest of its block
+ * of 32 (inputs 32 b to 32 b + 31), and to 2^-130: as precise as fp32 for that one,
+ * less for much smaller neighbours (a channel 1000 times the others costs its 31
+ * neighbours 10 of their bits); CGX_MX_FP4 or CGX_MX_FP6 x quantised as
  * cgx_mx_quantize_dev does.  Sums are held in fp32.  A row with a NaN or an
  * infinity gets NaN, as does every row's output of a weight block of byte 255.
  * Device pointers; M below 2^23, ldx and ldy below 2^32; no output or workspace may
@@ -512,7 +514,8 @@ int cgx_matmul_mx_dev(const float* x, size_t ldx, int M, const cgx_mx_weight* w,
                       float* y, size_t ldy, void* ws, size_t ws_bytes);
 
 /* Softmax cross entropy over the vocabulary of an lm_head W [K][V], from hidden
- * rows h [rows][K] (ldh floats apart), keeping no logits: with
+ * rows h [rows][K] (ldh floats apart), whose logits are not given back (small
+ * calls pass them through the workspace): with
  * z = h' W (h' as in cgx_matmul_mx_dev), lse[m] = log sum exp z[m] and
  * loss[m] = lse[m] - z[m][targets[m]], 0 for a target outside [0, V) (an
  * ignored row).  loss or lse may be NULL.  A row with a logit that is NaN or
@@ -520,7 +523,8 @@ int cgx_matmul_mx_dev(const float* x, size_t ldx, int M, const cgx_mx_weight* w,
  * The gradient: dh[m] (ldd apart) = dloss[m] (softmax(z[m]) - e_target) W^T,
  * with softmax(z) = exp(z - lse) for the lse that the first call wrote, dloss
  * [rows] the gradient of each row's loss (NULL: 1), and 0 for an ignored row;
- * a quantised h' passes its gradient on to h.  dh is written, not added to.
+ * a quantised h' passes its gradient on to h.  softmax - e_target is held as x' is in
+ * fp32, in blocks of 32 outputs.  dh is written, not added to.
  * ws: cgx_token_loss_mx_ws bytes (grad: 1 for the gradient, whose size is
  * enough for both calls), as in cgx_matmul_mx_dev, which says the rest; targets,
  * loss, lse and dloss are 4-byte aligned. */
